@@ -346,8 +346,8 @@ def _own(s):
     else:
         rc = lib.iris_b200_attention_blocks(
             s["out"].data_ptr(), case["heads"] * D, s["q"].data_ptr(), case["heads"] * D, s["k"].data_ptr(),
-            s["v"].data_ptr(), 2 * case["kv_heads"] * D, case["seq_q"], case["seq_k"], case["heads"], case["kv_heads"], D,
-            s["scale"], None if s["mask"] is None else s["mask"].data_ptr(), s["list"].data_ptr(), s["list"].shape[2],
+            2 * case["kv_heads"] * D, s["v"].data_ptr(), 2 * case["kv_heads"] * D, case["seq_q"], case["seq_k"], case["heads"],
+            case["kv_heads"], D, s["scale"], None if s["mask"] is None else s["mask"].data_ptr(), s["list"].data_ptr(), s["list"].shape[2],
             case["q_block"], case["k_block"], 0)
         out = s["out"]
     if rc:
