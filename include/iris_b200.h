@@ -354,6 +354,107 @@ int iris_b200_attention_kernel_for(const void *out, int ldo, const void *q, cons
                                    const void *v, int ldi, int heads, int kv_heads,
                                    int head_dim, int causal);
 
+/* ---- rotation from positions with several axes ----------------------------- */
+
+/* The prologue and the blocks above take cos / sin tables that the reference
+ * builds on the host, axis by axis (iris_transformer_flux.c and its siblings).
+ * These entry points start from the integer positions of the rows instead:
+ * pos [seq, n] (device), one column per axis (text, time, height, width, ...),
+ * any sign.
+ *
+ * A plan says how the pairs of a head turn: axis a (0 <= a < n) turns the next
+ * dim[a] dimensions (even, may be 0), pair i of them by
+ *     pos[s, a] * scale[a] * theta^(-2 i / dim[a]),
+ * or, with one_progression, pair j of the whole head by
+ *     pos[s, a(j)] * scale[a] * theta^(-2 j / head_dim).
+ * Dimensions behind the last axis are not turned. scale NULL: all 1. The plan
+ * lives in the caller's memory (no device memory, nothing to free) and can be
+ * used by any number of calls; its contents are the library's business.
+ * Angles are kept as 64-bit fractions of a turn, so that far positions lose
+ * nothing: cos and sin are within 2e-7 of the exact values for every int32
+ * position whose angle a double would resolve. Host arithmetic; needs no
+ * device. head_dim even, at most 512. */
+enum { IRIS_B200_ROPE_MAX_AXES = 8, IRIS_B200_ROPE_MAX_PAIRS = 256 };
+typedef struct iris_b200_rope_axes {
+    int n, head_dim;
+    uint64_t turn[IRIS_B200_ROPE_MAX_PAIRS];
+    uint8_t axis[IRIS_B200_ROPE_MAX_PAIRS];
+} iris_b200_rope_axes;
+int iris_b200_rope_axes_plan(iris_b200_rope_axes *axes, const int *dim, const double *scale, int n, double theta,
+                             int one_progression, int head_dim);
+
+/* cos_out / sin_out [seq, head_dim / 2] fp32: the tables that
+ * iris_dev_head_norm_rope, iris_b200_linear_qk_norm_rope and the block entry
+ * points take, built on the device. */
+int iris_b200_rope_axes_tables(float *cos_out, float *sin_out, const int *pos, const iris_b200_rope_axes *axes,
+                               int seq, int head_dim);
+
+/* iris_b200_qk_norm_rope without tables: q [seq, heads * head_dim] and k [seq,
+ * kv_heads * head_dim] (bf16, both with row stride ldi) are normalised per head
+ * (wq / wk [head_dim]; both NULL: no norm) and rotated by the row's positions
+ * into q_out (row stride ldqo) and k_out (ldko), in one pass. fp32 arithmetic,
+ * one rounding at the store. kv_heads may differ from heads (shared key
+ * heads); kv_heads 0: Q only, k and k_out are not looked at. In place: q_out
+ * == q with ldqo == ldi, and likewise k; outputs must not overlap the inputs
+ * in any other way. split_half: pairs (j, j + head_dim / 2) instead of (2 j, 2
+ * j + 1). The 16-byte kernel serves head_dim 64, 128 and 256 with strides in
+ * multiples of 8 and 16-byte aligned pointers; every other even head_dim up to
+ * 512 and alignment is served by a slower one. */
+int iris_b200_qk_norm_rope_axes(uint16_t *q_out, int ldqo, uint16_t *k_out, int ldko,
+                                const uint16_t *q, const uint16_t *k, int ldi,
+                                const float *wq, const float *wk, const int *pos,
+                                const iris_b200_rope_axes *axes, int seq, int heads, int kv_heads, int head_dim,
+                                float eps, int split_half);
+
+/* ---- attention over selected key blocks -------------------------------------- */
+
+/* Sequences of tens of thousands of image or video tokens spend nearly all
+ * their time in keys that hardly weigh. These three calls cut the key rows
+ * into blocks, score every block against every block of queries by the product
+ * of their means, and run the attention over the best blocks only. (No
+ * counterpart in the reference, whose attention is dense.) All of it runs on
+ * the library's stream, takes no scratch and keeps nothing between calls, so
+ * calls on different streams, and captured graphs of them, do not share
+ * anything but the caller's buffers. */
+
+/* means [nblocks, heads, head_dim] (fp32), nblocks = ceil(seq / block): mean of
+ * the rows x [seq, heads * head_dim] (bf16, row stride ldx) of every block;
+ * row_mask [seq] (NULL: all), 0 = the row is left out, whatever it holds.
+ * counts [nblocks] (may be NULL): the rows that counted. A block without any
+ * gets zeros. Blocks are independent: the means of a growing cache are kept up
+ * by calling this for the rows of its last block. */
+int iris_b200_block_means(float *means, int *counts, const uint16_t *x, int ldx, int seq, int heads, int head_dim,
+                          int block, const int *row_mask);
+
+/* list [heads, q_blocks, topk]: for every head and query block the key blocks
+ * to attend to, ascending, padded with -1. Score = q_means [q_blocks, heads,
+ * head_dim] . k_means [k_blocks, kv_heads, head_dim] in 64 bits, query head h
+ * against key head h / (heads / kv_heads). The first keep_first and the last
+ * keep_last blocks (text rows, the newest rows) are always taken, the rest of
+ * the topk places go to the highest scores, equal scores to the lowest block;
+ * a NaN ranks last. Blocks with k_counts [k_blocks] (NULL: all 1) zero are
+ * never taken. keep_first + keep_last <= topk; k_blocks <= 24576. */
+int iris_b200_block_select(int *list, const float *q_means, const float *k_means, const int *k_counts,
+                           int q_blocks, int k_blocks, int heads, int kv_heads, int head_dim,
+                           int topk, int keep_first, int keep_last);
+
+/* Scaled dot-product attention of each query over the rows of the key blocks
+ * listed for its query block: row r of head h reads list [heads, ceil(seq_q /
+ * q_block), list_len] at (h, r / q_block); entry b stands for the key rows [b *
+ * k_block, (b + 1) * k_block) below seq_k. Entries outside [0, ceil(seq_k /
+ * k_block)) are skipped, in any place; a block listed twice counts twice.
+ * key_mask [seq_k] (NULL: all): 0 = ignored key, whatever its K and V rows
+ * hold. A query without any key gets a zero row. Every tensor has its own row
+ * stride; query head h uses key head h / (heads / kv_heads). q_block 1 gives every query its own list. Not causal. kernel: one
+ * of IRIS_B200_KERNEL_*; the tcgen05 kernel serves head_dim 128, k_block 16,
+ * 32, 64 or a multiple of 128, strides in multiples of 8 and 16-byte aligned
+ * pointers, the general one everything up to head_dim 512. */
+int iris_b200_attention_blocks(uint16_t *out, int ldo, const uint16_t *q, int ldq,
+                               const uint16_t *k, int ldk, const uint16_t *v, int ldv,
+                               int seq_q, int seq_k, int heads, int kv_heads, int head_dim, float scale,
+                               const int *key_mask, const int *list, int list_len, int q_block, int k_block,
+                               int kernel);
+
 /* ---- multi-GPU decompositions (one process per GPU) ------------------------ */
 
 /* Heads [first, first + count) of rank `rank` when `heads` are split over

@@ -12,6 +12,11 @@ class IrisB200Error(RuntimeError):
     pass
 
 
+class RopeAxes(C.Structure):
+    """iris_b200_rope_axes of include/iris_b200.h."""
+    _fields_ = [("n", INT), ("head_dim", INT), ("turn", C.c_uint64 * 256), ("axis", C.c_uint8 * 256)]
+
+
 # name -> (restype, argtypes); one entry per declaration in include/*.h
 SIGNATURES = {
     # iris_dev.h
@@ -74,6 +79,14 @@ SIGNATURES = {
     "iris_b200_double_block": (INT, [VP, VP, VP, VP, VP, VP, INT, INT, INT, INT, INT, VP]),
     "iris_b200_attention_ex": (INT, [VP, INT, VP, VP, VP, INT, INT, INT, INT, INT, INT, FLT, INT, VP, INT]),
     "iris_b200_attention_kernel_for": (INT, [VP, INT, VP, VP, VP, INT, INT, INT, INT, INT]),
+    "iris_b200_rope_axes_plan": (INT, [C.POINTER(RopeAxes), VP, VP, INT, C.c_double, INT, INT]),
+    "iris_b200_rope_axes_tables": (INT, [VP, VP, VP, C.POINTER(RopeAxes), INT, INT]),
+    "iris_b200_qk_norm_rope_axes": (INT, [VP, INT, VP, INT, VP, VP, INT, VP, VP, VP, C.POINTER(RopeAxes), INT, INT, INT,
+                                          INT, FLT, INT]),
+    "iris_b200_block_means": (INT, [VP, VP, VP, INT, INT, INT, INT, INT, VP]),
+    "iris_b200_block_select": (INT, [VP, VP, VP, VP, INT, INT, INT, INT, INT, INT, INT, INT]),
+    "iris_b200_attention_blocks": (INT, [VP, INT, VP, INT, VP, INT, VP, INT, INT, INT, INT, INT, INT, FLT, VP, VP, INT, INT, INT,
+                                         INT]),
     "iris_b200_head_shard": (INT, [INT, INT, INT, C.POINTER(INT), C.POINTER(INT)]),
     "iris_b200_cfg_shard": (INT, [INT, INT, INT, INT, C.POINTER(INT), C.POINTER(INT), C.POINTER(INT), C.POINTER(INT)]),
     "iris_b200_seq_shard": (INT, [INT, INT, INT, C.POINTER(INT), C.POINTER(INT)]),
@@ -177,6 +190,16 @@ class Lib:
         if not p:
             raise IrisB200Error("iris_dev_alloc(%d) failed" % nbytes)
         return p
+
+    def rope_axes(self, dims, scales, theta, one_progression, head_dim):
+        """The rotation plan of iris_b200_rope_axes_plan."""
+        plan = RopeAxes()
+        n = len(dims)
+        rc = self.iris_b200_rope_axes_plan(plan, (INT * n)(*dims), (C.c_double * n)(*scales) if scales else None, n, theta,
+                                           int(one_progression), head_dim)
+        if rc:
+            raise IrisB200Error("iris_b200 error %d: %s" % (rc, self.iris_b200_strerror(rc).decode()))
+        return plan
 
     def to_device(self, arr):
         import numpy as np

@@ -182,6 +182,26 @@ void sm100_inject_stale_ticket(void);
 /* A device wait ran out: a ring that was in use cannot go on (multi_gpu.cu). */
 void ring_mark_failed(void);
 
+/* Attention over lists of key blocks (iris_b200_attention_blocks). */
+struct BlockAttnArgs {
+    uint16_t *out;
+    int ldo;
+    const uint16_t *q;
+    int ldq;
+    const uint16_t *k;
+    int ldk;
+    const uint16_t *v;
+    int ldv;
+    int seq_q, seq_k, heads, kv_heads, head_dim;
+    float scale;
+    const int *key_mask;
+    const int *list;            /* [heads, q_blocks, list_len] */
+    int list_len, q_block, k_block;
+    int q_blocks, k_blocks;
+};
+/* Per-device launch configuration is redone after a cleanup. */
+void block_select_release(void);
+
 /* Shared argument checks of the device-pointer attention entry points. */
 int check_attention_args(const char *op, const void *out, const void *q, const void *k, const void *v, int ldo,
                          int ldq, int ldkv, int seq_q, int seq_k, int heads, int kv_heads, int head_dim);

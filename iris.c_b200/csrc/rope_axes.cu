@@ -1,0 +1,440 @@
+/*
+ * Rotation from token positions with several axes (time, height, width, ...),
+ * as tables and inside the Q/K norm.
+ *
+ * Pair j of a head turns by p[s, axis(j)] * f_j. f_j / 2 pi is kept as a
+ * 64-bit fraction of a turn F_j, so the phase of a row is p * F_j modulo 2^64:
+ * whole turns fall off by themselves, for any sign and size of p, with an
+ * error of |p| 2^-65 turns; there is no range reduction and no table. Of the
+ * phase the top 32 bits are used (2^-32 turns = 1.5e-9 rad): the two highest
+ * give the quadrant after rounding, the rest an angle within pi / 4 on which
+ * the Taylor series of sine (to a^9) and cosine (to a^10) are within 2e-9 of
+ * the functions, below the rounding of fp32.
+ *
+ * k_rope_tables writes 8 bytes per pair and is bound by those stores.
+ *
+ * k_qk_norm_rope_axes reads and writes every element once and is bound by
+ * HBM. LANES = head_dim / 8 lanes own one (row, head) unit, 16 bytes each. A
+ * lane holds both members of its four pairs 4 l .. 4 l + 3 in either pairing
+ * (one 16-byte access, or two of 8 bytes half a head apart), so the rotation
+ * needs no exchange. A warp takes one row and a run of its heads: its lanes
+ * work out the head_dim / 2 sines and cosines of the row together, hand each
+ * other the four they need by shuffles, and fold them with the norm weights
+ * once per row.
+ */
+#include "common.cuh"
+
+#include <math.h>
+
+#include "iris_dev.h"
+
+namespace iris_b200 {
+namespace rope_axes {
+
+static constexpr int kThreads = 256;
+static constexpr int kInFlight = 4;          /* units of a lane group loaded before the first is used */
+static constexpr int kBlocksPerSM = 4;
+static constexpr int kMaxPairs = IRIS_B200_ROPE_MAX_PAIRS;
+
+struct Plan {
+    int n;                                   /* positions per row */
+    unsigned long long turn[kMaxPairs];      /* F_j */
+    unsigned char axis[kMaxPairs];
+};
+
+/* cos and sin of the phase p * turn. */
+__device__ __forceinline__ void turn_of(int p, unsigned long long turn, float &cs, float &sn) {
+    const uint32_t top = (uint32_t)(((unsigned long long)(long long)p * turn) >> 32);
+    const uint32_t quad = (top + 0x20000000u) >> 30;
+    const float a = (float)(int)(top - (quad << 30)) * 1.4629180792671596e-09f;     /* 2 pi / 2^32 */
+    const float b = a * a;
+    float s = fmaf(b, 1.0f / 362880.0f, -1.0f / 5040.0f);
+    s = fmaf(b, s, 1.0f / 120.0f);
+    s = fmaf(b, s, -1.0f / 6.0f);
+    s = fmaf(a * b, s, a);
+    float c = fmaf(b, -1.0f / 3628800.0f, 1.0f / 40320.0f);
+    c = fmaf(b, c, -1.0f / 720.0f);
+    c = fmaf(b, c, 1.0f / 24.0f);
+    c = fmaf(b, c, -0.5f);
+    c = fmaf(b, c, 1.0f);
+    const bool odd = quad & 1u;
+    const float x = odd ? s : c, y = odd ? c : s;
+    cs = __uint_as_float(__float_as_uint(x) ^ (((quad + 1u) & 2u) << 30));
+    sn = __uint_as_float(__float_as_uint(y) ^ ((quad & 2u) << 30));
+}
+
+/* ---- tables ---- */
+
+/* A thread keeps VEC consecutive pairs for all its rows. */
+template <int VEC>
+__global__ void __launch_bounds__(kThreads)
+k_rope_tables(float *__restrict__ cos_out, float *__restrict__ sin_out, const int *__restrict__ pos, int seq, int half,
+              const __grid_constant__ Plan plan) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int per_row = half / VEC, rows_per_block = kThreads / per_row;
+    const int r = threadIdx.x / per_row, j = (threadIdx.x - r * per_row) * VEC;
+    if (r >= rows_per_block) return;
+    unsigned long long turn[VEC];
+    int axis[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; i++) {
+        turn[i] = plan.turn[j + i];
+        axis[i] = plan.axis[j + i];
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (long long row = (long long)blockIdx.x * rows_per_block + r; row < seq; row += (long long)gridDim.x * rows_per_block) {
+        const int *p = pos + row * plan.n;
+        float c[VEC], s[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; i++) turn_of(__ldg(p + axis[i]), turn[i], c[i], s[i]);
+        float *co = cos_out + row * half + j, *so = sin_out + row * half + j;
+        if (VEC == 4) {
+            *reinterpret_cast<float4 *>(co) = make_float4(c[0], c[1 % VEC], c[2 % VEC], c[3 % VEC]);
+            *reinterpret_cast<float4 *>(so) = make_float4(s[0], s[1 % VEC], s[2 % VEC], s[3 % VEC]);
+        } else {
+            *co = c[0];
+            *so = s[0];
+        }
+    }
+}
+
+/* ---- norm and rotation ---- */
+
+struct Rows {
+    uint16_t *out[2];           /* Q, K */
+    const uint16_t *in[2];
+    const float *w[2];
+    int ldo[2];
+    int ldi;
+    int heads[2];
+    const int *pos;
+    int seq;
+    int chunk, chunks;          /* heads of a row per warp, warps per row */
+    float eps;
+};
+
+template <int HD, bool SPLIT, bool NORM>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSM)
+k_qk_norm_rope_axes(const __grid_constant__ Rows a, const __grid_constant__ Plan plan) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    constexpr int LANES = HD / 8;                   /* lanes of a unit */
+    constexpr int GROUPS = 32 / LANES;              /* units a warp works on at a time */
+    constexpr int PPL = HD / 64;                    /* pairs whose sine and cosine a lane works out */
+    const int lane = threadIdx.x & 31, l = lane & (LANES - 1), grp = lane / LANES;
+    /* The lane's pairs 4 l .. 4 l + 3 in memory. */
+    const int d0 = SPLIT ? 4 * l : 8 * l, d1 = SPLIT ? HD / 2 + 4 * l : 8 * l + 4;
+    unsigned long long turn[PPL];
+    int axis[PPL];
+#pragma unroll
+    for (int i = 0; i < PPL; i++) {
+        turn[i] = plan.turn[lane * PPL + i];
+        axis[i] = plan.axis[lane * PPL + i];
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const long long items = (long long)a.seq * a.chunks;
+    const long long warps = (long long)gridDim.x * (kThreads / 32);
+    for (long long item = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); item < items; item += warps) {
+        const int row = (int)(item / a.chunks);
+        const int u0 = (int)(item - (long long)row * a.chunks) * a.chunk;     /* first head, Q heads before K heads */
+        const int u1 = u0 + a.chunk;
+        float cs[4], sn[4];
+        {
+            float c[PPL], s[PPL];
+#pragma unroll
+            for (int i = 0; i < PPL; i++) turn_of(__ldg(a.pos + (size_t)row * plan.n + axis[i]), turn[i], c[i], s[i]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int src = (4 * l + i) / PPL;
+                cs[i] = __shfl_sync(0xffffffffu, c[i % PPL], src);
+                sn[i] = __shfl_sync(0xffffffffu, s[i % PPL], src);
+            }
+        }
+#pragma unroll
+        for (int part = 0; part < 2; part++) {
+            const int base = part ? a.heads[0] : 0;
+            const int h0 = (u0 > base ? u0 - base : 0), h1 = (u1 - base < a.heads[part] ? u1 - base : a.heads[part]);
+            if (h0 >= h1) continue;
+            /* Pair i of the lane is (x[i], x[4 + i]) with SPLIT, (x[2 i], x[2 i + 1]) without. */
+            float k00[4], k01[4], k10[4], k11[4];
+            if (NORM) {
+                const float4 w0 = __ldg(reinterpret_cast<const float4 *>(a.w[part] + d0));
+                const float4 w1 = __ldg(reinterpret_cast<const float4 *>(a.w[part] + d1));
+                const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float wa = w[SPLIT ? i : 2 * i], wb = w[SPLIT ? 4 + i : 2 * i + 1];
+                    k00[i] = cs[i] * wa;
+                    k01[i] = sn[i] * wb;
+                    k10[i] = cs[i] * wb;
+                    k11[i] = sn[i] * wa;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    k00[i] = k10[i] = cs[i];
+                    k01[i] = k11[i] = sn[i];
+                }
+            }
+            const uint16_t *in = a.in[part] + (size_t)row * a.ldi;
+            uint16_t *out = a.out[part] + (size_t)row * a.ldo[part];
+            for (int h = h0; h < h1; h += kInFlight * GROUPS) {
+                uint2 va[kInFlight], vb[kInFlight];
+#pragma unroll
+                for (int i = 0; i < kInFlight; i++) {
+                    const int hh = h + i * GROUPS + grp;
+                    va[i] = vb[i] = make_uint2(0u, 0u);
+                    if (hh < h1) {
+                        const uint16_t *src = in + hh * HD;
+                        if (SPLIT) {
+                            va[i] = *reinterpret_cast<const uint2 *>(src + d0);
+                            vb[i] = *reinterpret_cast<const uint2 *>(src + d1);
+                        } else {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(src + d0);
+                            va[i] = make_uint2(v.x, v.y);
+                            vb[i] = make_uint2(v.z, v.w);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kInFlight; i++) {
+                    const int hh = h + i * GROUPS + grp;
+                    float x[8] = {bf_lo(va[i].x), bf_hi(va[i].x), bf_lo(va[i].y), bf_hi(va[i].y),
+                                  bf_lo(vb[i].x), bf_hi(vb[i].x), bf_lo(vb[i].y), bf_hi(vb[i].y)};
+                    float inv = 1.0f;
+                    if (NORM) {
+                        float ss = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) ss = fmaf(x[j], x[j], ss);
+#pragma unroll
+                        for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                        inv = rsqrtf(ss * (1.0f / HD) + a.eps);
+                    }
+                    float y[8];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int ia = SPLIT ? j : 2 * j, ib = SPLIT ? 4 + j : 2 * j + 1;
+                        y[ia] = (x[ia] * k00[j] - x[ib] * k01[j]) * inv;
+                        y[ib] = (x[ib] * k10[j] + x[ia] * k11[j]) * inv;
+                    }
+                    if (hh < h1) {
+                        uint16_t *dst = out + hh * HD;
+                        const uint2 oa = make_uint2(cvt_bf16x2(y[0], y[1]), cvt_bf16x2(y[2], y[3]));
+                        const uint2 ob = make_uint2(cvt_bf16x2(y[4], y[5]), cvt_bf16x2(y[6], y[7]));
+                        if (SPLIT) {
+                            *reinterpret_cast<uint2 *>(dst + d0) = oa;
+                            *reinterpret_cast<uint2 *>(dst + d1) = ob;
+                        } else {
+                            *reinterpret_cast<uint4 *>(dst + d0) = make_uint4(oa.x, oa.y, ob.x, ob.y);
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+/* Any even head_dim up to 512, any alignment: one warp per (row, head), 2-byte
+ * accesses, every unit works out its own angles. */
+__global__ void __launch_bounds__(kThreads)
+k_qk_norm_rope_axes_any(const __grid_constant__ Rows a, const __grid_constant__ Plan plan, int head_dim, int split_half) {
+    const int lane = threadIdx.x & 31, half = head_dim / 2, per_row = a.heads[0] + a.heads[1];
+    const long long units = (long long)a.seq * per_row;
+    const long long warps = (long long)gridDim.x * (kThreads / 32);
+    for (long long unit = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); unit < units; unit += warps) {
+        const int row = (int)(unit / per_row), u = (int)(unit - (long long)row * per_row);
+        const int part = u >= a.heads[0], h = part ? u - a.heads[0] : u;
+        const uint16_t *in = a.in[part] + (size_t)row * a.ldi + (size_t)h * head_dim;
+        uint16_t *out = a.out[part] + (size_t)row * a.ldo[part] + (size_t)h * head_dim;
+        const float *w = a.w[part];
+        float inv = 1.0f;
+        if (w) {
+            float ss = 0.0f;
+            for (int d = lane; d < head_dim; d += 32) {
+                const float x = bf2f(in[d]);
+                ss = fmaf(x, x, ss);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            inv = rsqrtf(ss / head_dim + a.eps);
+        }
+        for (int j = lane; j < half; j += 32) {
+            const int i0 = split_half ? j : 2 * j, i1 = split_half ? j + half : 2 * j + 1;
+            float cs, sn;
+            turn_of(a.pos[(size_t)row * plan.n + plan.axis[j]], plan.turn[j], cs, sn);
+            const float x0 = bf2f(in[i0]) * (w ? inv * w[i0] : 1.0f), x1 = bf2f(in[i1]) * (w ? inv * w[i1] : 1.0f);
+            out[i0] = (uint16_t)cvt_bf16x2(x0 * cs - x1 * sn, 0.0f);
+            out[i1] = (uint16_t)cvt_bf16x2(x1 * cs + x0 * sn, 0.0f);
+        }
+    }
+}
+
+static int bad(const char *op, const char *why) {
+    set_error(IRIS_B200_EINVAL, op, why);
+    return IRIS_B200_EINVAL;
+}
+
+/* The caller's plan, checked again: it lives in the caller's memory. */
+static bool plan_of(const iris_b200_rope_axes *axes, int head_dim, Plan *plan) {
+    if (!axes || head_dim <= 0 || (head_dim & 1) || head_dim / 2 > kMaxPairs || axes->head_dim != head_dim || axes->n < 1 ||
+        axes->n > IRIS_B200_ROPE_MAX_AXES)
+        return false;
+    plan->n = axes->n;
+    for (int j = 0; j < head_dim / 2; j++) {
+        if (axes->axis[j] >= axes->n) return false;
+        plan->turn[j] = axes->turn[j];
+        plan->axis[j] = axes->axis[j];
+    }
+    return true;
+}
+
+static bool aligned(const void *p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+template <int HD>
+static cudaError_t launch_rows(const cudaLaunchConfig_t &cfg, const Rows &a, const Plan &plan, bool split, bool norm) {
+    if (split)
+        return norm ? cudaLaunchKernelEx(&cfg, k_qk_norm_rope_axes<HD, true, true>, a, plan)
+                    : cudaLaunchKernelEx(&cfg, k_qk_norm_rope_axes<HD, true, false>, a, plan);
+    return norm ? cudaLaunchKernelEx(&cfg, k_qk_norm_rope_axes<HD, false, true>, a, plan)
+                : cudaLaunchKernelEx(&cfg, k_qk_norm_rope_axes<HD, false, false>, a, plan);
+}
+
+/* Launch with programmatic stream serialisation (the kernels wait for the
+ * grid ahead before they touch memory that it may have written). */
+struct Launch {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    Launch(unsigned blocks) : cfg(), attr() {
+        cfg.gridDim = dim3(blocks);
+        cfg.blockDim = dim3(kThreads);
+        cfg.stream = g.stream;
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+    }
+};
+
+}  // namespace rope_axes
+}  // namespace iris_b200
+
+using namespace iris_b200;
+using namespace iris_b200::rope_axes;
+
+extern "C" int iris_b200_rope_axes_plan(iris_b200_rope_axes *axes, const int *dim, const double *scale, int n, double theta,
+                                        int one_progression, int head_dim) {
+    const char *op = "rope_axes_plan";
+    if (!axes || !dim || n < 1 || n > IRIS_B200_ROPE_MAX_AXES || head_dim <= 0 || (head_dim & 1) || head_dim / 2 > kMaxPairs)
+        return bad(op, "bad argument");
+    if (!(theta > 0.0) || !isfinite(theta)) return bad(op, "theta must be positive");
+    long long sum = 0;
+    for (int a = 0; a < n; a++) {
+        if (dim[a] < 0 || (dim[a] & 1)) return bad(op, "an axis turns an even number of dimensions");
+        if (scale && !isfinite(scale[a])) return bad(op, "scales must be finite");
+        sum += dim[a];
+    }
+    if (sum > head_dim) return bad(op, "the axes turn more dimensions than a head has");
+    axes->n = n;
+    axes->head_dim = head_dim;
+    int j = 0;
+    for (int a = 0; a < n; a++)
+        for (int i = 0; i < dim[a] / 2; i++, j++) {
+            const long double power = one_progression ? 2.0L * j / head_dim : 2.0L * i / dim[a];
+            const long double turns = (long double)(scale ? scale[a] : 1.0) * powl((long double)theta, -power) /
+                                      6.283185307179586476925286766559L;
+            long double frac = turns - floorl(turns);
+            if (!(frac >= 0.0L) || frac >= 1.0L) frac = 0.0L;
+            axes->turn[j] = (uint64_t)(frac * 18446744073709551616.0L);
+            axes->axis[j] = (uint8_t)a;
+        }
+    for (; j < IRIS_B200_ROPE_MAX_PAIRS; j++) {
+        axes->turn[j] = 0;
+        axes->axis[j] = 0;
+    }
+    return IRIS_B200_OK;
+}
+
+extern "C" int iris_b200_rope_axes_tables(float *cos_out, float *sin_out, const int *pos, const iris_b200_rope_axes *axes,
+                                          int seq, int head_dim) {
+    const char *op = "rope_axes_tables";
+    Plan plan;
+    if (seq < 0 || !plan_of(axes, head_dim, &plan)) return bad(op, "bad argument");
+    if (seq > 0 && (!cos_out || !sin_out || !pos)) return bad(op, "bad argument");
+    if (!require_device(op)) return IRIS_B200_ENODEV;
+    if (seq == 0) return IRIS_B200_OK;
+    const int half = head_dim / 2;
+    const bool vec = half % 4 == 0 && aligned(cos_out, 16) && aligned(sin_out, 16);
+    const int rows_per_block = kThreads / (vec ? half / 4 : half);
+    long long blocks = ((long long)seq + rows_per_block - 1) / rows_per_block;
+    if (blocks > (long long)g.sm_count * 8) blocks = (long long)g.sm_count * 8;
+    Launch l((unsigned)blocks);
+    const cudaError_t err = vec ? cudaLaunchKernelEx(&l.cfg, k_rope_tables<4>, cos_out, sin_out, pos, seq, half, plan)
+                                : cudaLaunchKernelEx(&l.cfg, k_rope_tables<1>, cos_out, sin_out, pos, seq, half, plan);
+    g.launches++;
+    return cuda_ok(err, op) ? IRIS_B200_OK : IRIS_B200_ECUDA;
+}
+
+extern "C" int iris_b200_qk_norm_rope_axes(uint16_t *q_out, int ldqo, uint16_t *k_out, int ldko, const uint16_t *q,
+                                           const uint16_t *k, int ldi, const float *wq, const float *wk, const int *pos,
+                                           const iris_b200_rope_axes *axes, int seq, int heads, int kv_heads, int head_dim,
+                                           float eps, int split_half) {
+    const char *op = "qk_norm_rope_axes";
+    Plan plan;
+    if (seq < 0 || heads <= 0 || kv_heads < 0 || !plan_of(axes, head_dim, &plan)) return bad(op, "bad argument");
+    const bool has_k = kv_heads > 0;
+    if ((long long)heads * head_dim > ldi || (long long)kv_heads * head_dim > ldi || (long long)heads * head_dim > ldqo ||
+        (has_k && (long long)kv_heads * head_dim > ldko))
+        return bad(op, "a row stride is shorter than a row of heads");
+    if ((wq != NULL) != (wk != NULL) && has_k) return bad(op, "norm weights for one of Q and K only");
+    if (!(eps >= 0.0f)) return bad(op, "eps must not be negative");
+    if (seq > 0 && (!q_out || !q || !pos || (has_k && (!k_out || !k)))) return bad(op, "bad argument");
+    /* In place means the same rows; anything else that overlaps would be read after it is written. */
+    if (seq > 0 && ((q_out == q && ldqo != ldi) || (has_k && k_out == k && ldko != ldi)))
+        return bad(op, "in place needs equal row strides");
+    if (!require_device(op)) return IRIS_B200_ENODEV;
+    if (seq == 0) return IRIS_B200_OK;
+    Rows a = {};
+    a.out[0] = q_out;
+    a.in[0] = q;
+    a.w[0] = wq;
+    a.ldo[0] = ldqo;
+    a.heads[0] = heads;
+    if (has_k) {
+        a.out[1] = k_out;
+        a.in[1] = k;
+        a.w[1] = wk;
+        a.ldo[1] = ldko;
+        a.heads[1] = kv_heads;
+    }
+    a.ldi = ldi;
+    a.pos = pos;
+    a.seq = seq;
+    a.eps = eps;
+    const int per_row = heads + kv_heads;
+    const bool fast = (head_dim == 64 || head_dim == 128 || head_dim == 256) && ldi % 8 == 0 && ldqo % 8 == 0 &&
+                      aligned(q, 16) && aligned(q_out, 16) && (!wq || aligned(wq, 16)) &&
+                      (!has_k || (ldko % 8 == 0 && aligned(k, 16) && aligned(k_out, 16) && (!wk || aligned(wk, 16))));
+    if (!fast) {
+        long long blocks = ((long long)seq * per_row + kThreads / 32 - 1) / (kThreads / 32);
+        if (blocks > (long long)g.sm_count * 32) blocks = (long long)g.sm_count * 32;
+        k_qk_norm_rope_axes_any<<<(unsigned)blocks, kThreads, 0, g.stream>>>(a, plan, head_dim, split_half);
+        return after_launch(op) ? IRIS_B200_OK : IRIS_B200_ECUDA;
+    }
+    /* A row is cut into as many warps as it takes to fill the device once. */
+    const long long slots = (long long)g.sm_count * kBlocksPerSM * (kThreads / 32);
+    const int groups = 32 / (head_dim / 8);
+    int chunks = (int)((slots + seq - 1) / seq);
+    const int most = (per_row + groups - 1) / groups;
+    if (chunks > most) chunks = most;
+    a.chunk = (per_row + chunks - 1) / chunks;
+    a.chunk = (a.chunk + groups - 1) / groups * groups;
+    a.chunks = (per_row + a.chunk - 1) / a.chunk;
+    long long blocks = ((long long)seq * a.chunks + kThreads / 32 - 1) / (kThreads / 32);
+    if (blocks > (long long)g.sm_count * kBlocksPerSM) blocks = (long long)g.sm_count * kBlocksPerSM;
+    Launch l((unsigned)blocks);
+    const bool split = split_half != 0, norm = wq != NULL;
+    const cudaError_t err = head_dim == 64    ? launch_rows<64>(l.cfg, a, plan, split, norm)
+                            : head_dim == 128 ? launch_rows<128>(l.cfg, a, plan, split, norm)
+                                              : launch_rows<256>(l.cfg, a, plan, split, norm);
+    g.launches++;
+    return cuda_ok(err, op) ? IRIS_B200_OK : IRIS_B200_ECUDA;
+}
