@@ -88,7 +88,7 @@ k_attention_blocks_any(const BlockAttnArgs a, int tiles_per_block) {
             l = l * alpha + ps;
             m = mnew;
             /* The probabilities meet V as bf16, as in the tensor-core kernel; their sum keeps fp32. */
-            const float pb = bf2f(f2bf(p));
+            const float pb = bf_lo(cvt_bf16x2(p, 0.0f));
 #pragma unroll
             for (int t = 0; t < kMaxHeadDim / 32; t++) acc[t] *= alpha;
             for (int j = 0; j < kKeysPerTile; j++) {
@@ -103,7 +103,7 @@ k_attention_blocks_any(const BlockAttnArgs a, int tiles_per_block) {
         }
     }
     if (!qvalid) return;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
     for (int t = 0; t < kMaxHeadDim / 32; t++) {
         const int d = lane + 32 * t;
@@ -179,11 +179,12 @@ extern "C" int iris_b200_attention_blocks(uint16_t *out, int ldo, const uint16_t
     a.k_block = k_block;
     a.q_blocks = (int)(((long long)seq_q + q_block - 1) / q_block);
     a.k_blocks = (int)(((long long)seq_k + k_block - 1) / k_block);
-    if (kernel == IRIS_B200_KERNEL_TCGEN05) {
+    const bool fast = attention_blocks_sm100_supported(a);
+    if (kernel == IRIS_B200_KERNEL_TCGEN05 && !fast) {
         set_error(IRIS_B200_EUNSUPPORTED, op, "arguments outside the tcgen05 kernel's domain");
         return IRIS_B200_EUNSUPPORTED;
     }
     if (!require_device(op)) return IRIS_B200_ENODEV;
     if (seq_q == 0) return IRIS_B200_OK;
-    return launch_any(a);
+    return fast && kernel != IRIS_B200_KERNEL_GENERIC ? launch_attention_blocks_sm100(a) : launch_any(a);
 }

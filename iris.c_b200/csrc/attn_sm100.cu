@@ -76,6 +76,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include "attn_tc.cuh"
 #include "kernels.h"
 #include "tc_ptx.cuh"
 #include <math.h>
@@ -169,26 +170,6 @@ struct Params {
                                   3: merge with the state and write the final bf16 output */
 };
 
-/* ---------------- bounded waits ---------------- */
-
-struct Ctx {
-    uint32_t bars;                  /* shared address of the barrier block */
-    volatile uint32_t *abort_flag;  /* generic pointer to the CTA abort word */
-    unsigned int *status;
-    unsigned long long wait_ns;
-};
-
-/* A wait ran out: raise the CTA's abort flag and record the first such event
- * of the launch in the device status word. */
-__device__ __forceinline__ void give_up(const Ctx &c, int site, unsigned aux) {
-    *c.abort_flag = 1u;
-    if (atomicCAS(c.status, 0u, 1u) == 0u) {
-        c.status[1] = (unsigned)site;
-        c.status[2] = blockIdx.x;
-        c.status[3] = aux;
-    }
-}
-
 /* Self-checks of the -DIRIS_B200_CHECK build (tile and slot indices, scratch
  * capacities, rows handed to TMA): a violated check never traps; it records
  * the first site in words 4-7 of the status word, which
@@ -209,27 +190,6 @@ __device__ __noinline__ void check_failed(unsigned int *status, int site, unsign
 #else
 #define IRIS_CHECK(status, cond, site, aux) ((void)0)
 #endif
-
-/* Bounded wait. Returns false when the CTA is aborting. `site` identifies
- * the caller in the status word. */
-__device__ __forceinline__ bool mbar_wait_slow(const Ctx &c, uint32_t bar, uint32_t parity, int site) {
-    unsigned long long t0 = global_ns();
-    for (uint32_t spin = 0;; spin++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((spin & 63u) == 63u) {
-            if (*c.abort_flag) return false;
-            if (global_ns() - t0 > c.wait_ns || spin > (1u << 26)) {
-                give_up(c, site, parity);
-                return false;
-            }
-        }
-    }
-}
-__device__ __forceinline__ bool mbar_wait(const Ctx &c, int idx, uint32_t parity, int site) {
-    uint32_t bar = c.bars + idx * 8;
-    if (mbar_try_wait(bar, parity)) return true;
-    return mbar_wait_slow(c, bar, parity, site);
-}
 
 /* Bounded wait for a 32-bit word in global memory that somebody else (another
  * CTA, a copy engine, another GPU) advances to at least `target`. */
@@ -531,33 +491,6 @@ __device__ __forceinline__ void tile_bits(const Params &p, int j, int nkeys, uin
         uint32_t b = left >= 32 ? 0xFFFFFFFFu : (left <= 0 ? 0u : ((1u << left) - 1u));
         if (p.mask_bits) b &= p.mask_bits[j * 4 + w];    /* padded to whole tiles by the packer */
         bits[w] = b;
-    }
-}
-
-/* Scores of masked / out-of-range keys become -inf. */
-__device__ __forceinline__ void mask_chunk(uint32_t *v, uint32_t bits) {
-#pragma unroll
-    for (int i = 0; i < 32; i++)
-        if (!((bits >> i) & 1u)) v[i] = 0xFF800000u;
-}
-
-/* Half an S row (64 scores) -> P (bf16 pairs into 32 columns at tP) and the
- * four partial row sums: one fp32 exponential per score. */
-__device__ __forceinline__ void exp_half(const uint32_t *s, float sl2, float neg_ref, float *sum4, uint32_t tP) {
-#pragma unroll
-    for (int ch = 0; ch < 2; ch++) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float x0 = fmaf(__uint_as_float(s[ch * 32 + 2 * i]), sl2, neg_ref);
-            float x1 = fmaf(__uint_as_float(s[ch * 32 + 2 * i + 1]), sl2, neg_ref);
-            float p0 = ex2(x0);
-            float p1 = ex2(x1);
-            sum4[(2 * i) & 3] += p0;
-            sum4[(2 * i + 1) & 3] += p1;
-            pk[i] = cvt_bf16x2(p0, p1);
-        }
-        tmem_st16(tP + ch * 16, pk);
     }
 }
 

@@ -199,8 +199,12 @@ struct BlockAttnArgs {
     int list_len, q_block, k_block;
     int q_blocks, k_blocks;
 };
+/* Whether the tensor-core kernel takes these arguments, and its launch. */
+bool attention_blocks_sm100_supported(const BlockAttnArgs &a);
+int launch_attention_blocks_sm100(const BlockAttnArgs &a);
 /* Per-device launch configuration is redone after a cleanup. */
 void block_select_release(void);
+void attention_blocks_release(void);
 
 /* Shared argument checks of the device-pointer attention entry points. */
 int check_attention_args(const char *op, const void *out, const void *q, const void *k, const void *v, int ldo,

@@ -137,6 +137,7 @@ void iris_dev_cleanup(void) {
     cuda_ok(cudaStreamSynchronize(g.stream), "sync");
     sm100_release();
     block_select_release();
+    attention_blocks_release();
     if (g.scratch) cuda_ok(cudaFree(g.scratch), "free");
     g.scratch = NULL;
     g.scratch_bytes = 0;

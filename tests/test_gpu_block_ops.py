@@ -383,6 +383,47 @@ def test_attention_general_kernel(lib, sq, sk, heads, kv, hd, n, qb, kb, masked,
     check_attention(lib, sq, sk, heads, kv, hd, n, qb, kb, AUTO, masked, pad, junk, seed=5)
 
 
+TENSOR = [  # sq, sk, heads, kv, list_len, q_block, k_block, masked, pad, junk
+    (1, 1, 1, 1, 1, 1, 64, False, 0, False), (128, 128, 1, 1, 1, 128, 128, False, 0, False), (128, 128, 2, 2, 2, 128, 64, False, 8, False),
+    (129, 200, 2, 1, 3, 128, 64, True, 0, False), (300, 333, 3, 3, 4, 128, 64, True, 16, True), (300, 333, 3, 3, 20, 128, 16, True, 0, True),
+    (517, 517, 2, 2, 9, 256, 32, True, 0, True), (260, 900, 4, 2, 2, 384, 256, True, 0, True), (64, 700, 2, 2, 3, 100, 128, True, 0, False),
+    (77, 2000, 2, 2, 2, 16, 512, True, 0, False), (3, 4096, 4, 1, 64, 1, 64, True, 0, True), (2, 8192, 2, 1, 32, 2, 256, False, 0, False),
+    (1, 4096, 8, 2, 40, 1, 64, False, 0, False), (40, 3000, 2, 2, 47, 40, 64, True, 0, True), (128, 3000, 1, 1, 33, 128, 64, True, 0, True)]
+
+
+@pytest.mark.parametrize("sq,sk,heads,kv,n,qb,kb,masked,pad,junk", TENSOR)
+def test_attention_tensor_kernel(lib, sq, sk, heads, kv, n, qb, kb, masked, pad, junk):
+    check_attention(lib, sq, sk, heads, kv, 128, n, qb, kb, TCGEN05, masked, pad, junk)
+    check_attention(lib, sq, sk, heads, kv, 128, n, qb, kb, TCGEN05, masked, pad, junk, seed=7, gain=3.0)
+
+
+@pytest.mark.parametrize("sq,heads,n", [(1, 8, 40), (300, 3, 6), (100, 2, 40)])
+def test_attention_tensor_kernel_growing_scores(lib, sq, heads, n):
+    """Scores that rise from block to block, so that the running maximum moves and O is rescaled."""
+    sk, kb = 2560, 64
+    q = torch.ones(sq, heads * 128) + 0.1 * randn(1, sq, heads * 128)
+    k = (torch.arange(sk).reshape(sk, 1) // kb * 0.02 - 0.3) + 0.05 * randn(2, sk, heads * 128)
+    v = randn(3, sk, heads * 128)
+    q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+    lists = random_lists(4, heads, -(-sq // 128), sk // kb, n)
+    got = run_attention(lib, q, k, v, heads, heads, 128, None, lists, 128, kb, TCGEN05, scale=0.5)
+    want, mag = ref.attention(q, k, v, heads, heads, 128, 0.5, None, lists, 128, kb)
+    # |s| up to 64 * 0.5 = 32 here: a dot product of magnitude 64 off by 2^-17 relative, 2^-10 in s
+    assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -10) * mag).all()
+
+
+def test_attention_values_that_are_not_finite_show(lib):
+    """A NaN in a key or value row that counts reaches the rows that see it, and no others."""
+    q, k, v = (randn(i, 256, 128).bfloat16() for i in range(3))
+    v[70, 5] = NAN
+    k[200] = NAN
+    lists = torch.tensor([[[0, 1], [2, 3]]], dtype=torch.int32)
+    for kernel in (GENERIC, TCGEN05):
+        got = run_attention(lib, q, k, v, 1, 1, 128, None, lists, 128, 64, kernel)
+        bad = got.isnan()
+        assert bad[:128, 5].all() and bad[:128].sum() == 128 and bad[128:].all()
+
+
 @pytest.mark.parametrize("kernel", [GENERIC, AUTO])
 def test_attention_rows_without_keys(lib, kernel):
     q, k, v = (randn(i, r, 256).bfloat16() for i, r in enumerate((300, 200, 200)))
