@@ -433,7 +433,8 @@ int iris_b200_block_means(float *means, int *counts, const uint16_t *x, int ldx,
  * keep_last blocks (text rows, the newest rows) are always taken, the rest of
  * the topk places go to the highest scores, equal scores to the lowest block;
  * a NaN ranks last. Blocks with k_counts [k_blocks] (NULL: all 1) zero are
- * never taken. keep_first + keep_last <= topk; k_blocks <= 24576. */
+ * never taken. keep_first + keep_last <= topk; k_blocks <= 23552; head_dim <=
+ * 512. */
 int iris_b200_block_select(int *list, const float *q_means, const float *k_means, const int *k_counts,
                            int q_blocks, int k_blocks, int heads, int kv_heads, int head_dim,
                            int topk, int keep_first, int keep_last);

@@ -10,20 +10,23 @@
  *
  * k_block_select scores in fp64: a product of two fp32 means is exact there,
  * and a list only depends on the order of summation where two scores agree to
- * 1e-16. Rows of a score tile are eight (query block, head) pairs of one key
- * head; the products run on the fp64 matrix instruction (m8n8k4), whose
- * operand fragments are read straight from the fp32 means: the summation
- * index may be permuted as long as both operands agree, so a lane takes four
- * consecutive dimensions with one 16-byte load and no shared memory is needed.
- * The scores become order-preserving 64-bit keys in shared memory; a warp then
- * finds the topk-th largest key of a row by bisection over its bits and writes
- * the chosen blocks in ascending order, equal keys from the lowest index.
+ * 1e-16. Up to sixteen (query block, head) rows of one key head share a score
+ * tile on the fp64 matrix instruction (m8n8k4). Its key operand is read
+ * straight from the fp32 means: the summation index may be permuted as long as
+ * both operands agree, so a lane takes four consecutive dimensions with one
+ * 16-byte load and all loads of a tile are in flight together. The scores
+ * become order-preserving 64-bit keys in shared memory. Where there are few
+ * rows, the blocks are cut over the CTAs of a cluster, which send the keys to
+ * the CTA that chooses for the row. One to eight warps then find the topk-th
+ * largest key of a row by a search over its bits and write the chosen blocks
+ * in ascending order, equal keys from the lowest index.
  */
 #include "common.cuh"
 
 #include <limits.h>
 
 #include "iris_dev.h"
+#include "tc_ptx.cuh"
 
 namespace iris_b200 {
 namespace block_select {
@@ -107,8 +110,12 @@ k_block_means(float *__restrict__ means, int *__restrict__ counts, const uint16_
 /* ---- lists ---- */
 
 static constexpr int kSelThreads = 256;
-static constexpr int kSelRows = 8;               /* (query block, head) rows of a CTA */
-static constexpr int kMaxBlocks = 24576;         /* 64-bit keys of one row in shared memory */
+static constexpr int kSelWarps = kSelThreads / 32;
+static constexpr int kSelRows = 16;              /* (query block, head) rows of a cluster: two score tiles of eight */
+static constexpr int kMaxCtas = 8;               /* CTAs of a cluster, each with a slice of the blocks */
+static constexpr int kMaxBlocks = 23552;         /* 64-bit keys of one row in shared memory */
+static constexpr int kMaxHeadDim = 512;
+static constexpr int kSelSmem = kMaxBlocks * 8 + kMaxHeadDim * 64;      /* one row's keys, one tile of rows */
 
 struct Select {
     int *list;
@@ -117,7 +124,11 @@ struct Select {
     int q_blocks, k_blocks, heads, kv_heads, head_dim;
     int group;                  /* query heads of a key head */
     int topk, keep_first, keep_last;
-    int rows;                   /* rows of a CTA: kSelRows, or fewer where their keys would not fit */
+    int rows;                   /* rows of a cluster */
+    int ctas, slice;            /* CTAs of a cluster, blocks of each (a multiple of 8) */
+    int own_rows;               /* rows whose keys a CTA holds: ceil(rows / ctas) */
+    int team;                   /* warps that choose for one row */
+    int steps;                  /* products of four dimensions: head_dim rounded up to 16, / 4 */
 };
 
 __device__ __forceinline__ unsigned long long key_of(double s) {
@@ -128,7 +139,7 @@ __device__ __forceinline__ unsigned long long key_of(double s) {
 }
 
 /* Row r of key head g: the query block and head. Rows run over the heads of
- * the group inside a query block, so the lists of a tile lie close together. */
+ * the group inside a query block. */
 __device__ __forceinline__ bool row_of(const Select &p, int g, long long r, int *qb, int *head) {
     if (r >= (long long)p.q_blocks * p.group) return false;
     *qb = (int)(r / p.group);
@@ -136,125 +147,328 @@ __device__ __forceinline__ bool row_of(const Select &p, int g, long long r, int 
     return true;
 }
 
-/* Scores of the rows r0 .. r0 + 7 of key head g against the blocks j0 .. j0 + 7
- * by one warp: two fp64 values per lane, row lane / 4, blocks j0 + 2 (lane & 3)
- * and the next. VEC: four consecutive dimensions per lane and step. */
-template <bool VEC>
-__device__ __forceinline__ void score_tile(const Select &p, const float *qrow, const float *krow, int lane, double d[2]) {
-    d[0] = d[1] = 0.0;
-    for (int k0 = 0; k0 < p.head_dim; k0 += 16) {
-        const int e = k0 + (lane & 3) * 4;
-        float a[4] = {0.0f, 0.0f, 0.0f, 0.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (VEC) {
-            if (qrow) {
-                const float4 v = __ldg(reinterpret_cast<const float4 *>(qrow + e));
-                a[0] = v.x; a[1] = v.y; a[2] = v.z; a[3] = v.w;
-            }
-            if (krow) {
-                const float4 v = __ldg(reinterpret_cast<const float4 *>(krow + e));
-                b[0] = v.x; b[1] = v.y; b[2] = v.z; b[3] = v.w;
-            }
-        } else {
+__device__ __forceinline__ void mma_f64(double d[2], double a, double b) {
+    asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+                 : "+d"(d[0]), "+d"(d[1]) : "d"(a), "d"(b));
+}
+
+/* Scores of the cluster's rows against the blocks j0 .. j0 + 7 by one warp:
+ * d[m] holds row 8 m + lane / 4 and the blocks j0 + 2 (lane & 3), + 1. Product
+ * s of a 16-dimension group takes the dimensions 16 g + 4 (lane & 3) + s. qf:
+ * the rows as fp64 operand fragments in shared memory. HD 0: any head_dim. */
+template <int HD>
+__device__ __forceinline__ void score_tile(const Select &p, const double *qf, const float *krow, int lane, int tiles, double d[2][2]) {
+    d[0][0] = d[0][1] = d[1][0] = d[1][1] = 0.0;
+    const int e0 = (lane & 3) * 4;
+    if (HD > 0) {
+        float4 k[HD / 16 + 1];
+#pragma unroll
+        for (int g = 0; g < HD / 16; g++)
+            k[g] = krow ? __ldg(reinterpret_cast<const float4 *>(krow + 16 * g + e0)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int g = 0; g < HD / 16; g++) {
+            const float b[4] = {k[g].x, k[g].y, k[g].z, k[g].w};
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (qrow && e + i < p.head_dim) a[i] = qrow[e + i];
-                if (krow && e + i < p.head_dim) b[i] = krow[e + i];
+                const double bv = (double)b[i];
+                mma_f64(d[0], qf[(4 * g + i) * 32 + lane], bv);
+                if (tiles > 1) mma_f64(d[1], qf[(p.steps + 4 * g + i) * 32 + lane], bv);
             }
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const double av = (double)a[i], bv = (double)b[i];
-            asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
-                         : "+d"(d[0]), "+d"(d[1]) : "d"(av), "d"(bv));
+    } else {
+        for (int s = 0; s < p.steps; s++) {
+            const int e = (s >> 2) * 16 + e0 + (s & 3);
+            const double bv = krow && e < p.head_dim ? (double)krow[e] : 0.0;
+            mma_f64(d[0], qf[s * 32 + lane], bv);
+            if (tiles > 1) mma_f64(d[1], qf[(p.steps + s) * 32 + lane], bv);
         }
     }
 }
 
-/* The list of one row by one warp: the keys of all blocks are in shared
- * memory (0: not eligible, all ones: always taken). */
-__device__ __forceinline__ void choose(const Select &p, const unsigned long long *keys, int *list, int lane) {
-    int eligible = 0;
-    unsigned long long hi = 0ull, lo = ~0ull;
-    for (int j = lane; j < p.k_blocks; j += 32) {
+/* A team of p.team warps works on one row; `me` is the warp's place in it. */
+struct Team {
+    int me, warps, barrier;
+    unsigned *counts;           /* [2][kSelWarps][2] shared words of this team */
+    unsigned turn;
+    __device__ __forceinline__ void sync() const {
+        if (warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(warps * 32) : "memory");
+    }
+    /* The team's sums of two words, and what the warps before this one add to them. */
+    __device__ __forceinline__ void sum(unsigned &a, unsigned &b, unsigned &a_before, unsigned &b_before) {
+        a = __reduce_add_sync(0xffffffffu, a);
+        b = __reduce_add_sync(0xffffffffu, b);
+        a_before = b_before = 0u;
+        if (warps == 1) return;
+        unsigned *c = counts + (turn++ & 1u) * (2 * kSelWarps);
+        if ((threadIdx.x & 31) == 0) {
+            c[2 * me] = a;
+            c[2 * me + 1] = b;
+        }
+        sync();
+        a = b = 0u;
+        for (int w = 0; w < warps; w++) {
+            if (w == me) {
+                a_before = a;
+                b_before = b;
+            }
+            a += c[2 * w];
+            b += c[2 * w + 1];
+        }
+    }
+    /* The team's maxima of two words. */
+    __device__ __forceinline__ void most(unsigned &a, unsigned &b) {
+        a = __reduce_max_sync(0xffffffffu, a);
+        b = __reduce_max_sync(0xffffffffu, b);
+        if (warps == 1) return;
+        unsigned *c = counts + (turn++ & 1u) * (2 * kSelWarps);
+        if ((threadIdx.x & 31) == 0) {
+            c[2 * me] = a;
+            c[2 * me + 1] = b;
+        }
+        sync();
+        for (int w = 0; w < warps; w++) {
+            a = c[2 * w] > a ? c[2 * w] : a;
+            b = c[2 * w + 1] > b ? c[2 * w + 1] : b;
+        }
+    }
+    /* The smallest of lo and the largest of hi over the team: high words, then the low words that go with them. */
+    __device__ __forceinline__ void span(unsigned long long &lo, unsigned long long &hi) {
+        unsigned h = (unsigned)(hi >> 32), l = ~(unsigned)(lo >> 32);
+        most(h, l);
+        unsigned h2 = (unsigned)(hi >> 32) == h ? (unsigned)hi : 0u, l2 = ~(unsigned)(lo >> 32) == l ? ~(unsigned)lo : 0u;
+        most(h2, l2);
+        hi = (unsigned long long)h << 32 | h2;
+        lo = (unsigned long long)~l << 32 | ~l2;
+    }
+};
+
+static constexpr int kBins = 256;
+/* Bin of a score: (float)kBins / range may round up, hence the limit. Monotone: each operation rounds monotonically. */
+__device__ __forceinline__ int bin_of(float f, float low, float per) {
+    const int b = (int)((f - low) * per);
+    return b < kBins - 1 ? b : kBins - 1;
+}
+
+/* The score of a key that is neither 0 nor all ones, to fp32: keeps the order. */
+__device__ __forceinline__ float score_of(unsigned long long key) {
+    return (float)__longlong_as_double((long long)((key >> 63) ? key & 0x7FFFFFFFFFFFFFFFull : ~key));
+}
+__device__ __forceinline__ uint32_t ordered(float f) {
+    const uint32_t b = __float_as_uint(f);
+    return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t b) { return __uint_as_float((b >> 31) ? b & 0x7FFFFFFFu : ~b); }
+
+/* The list of one row: its keys (0: not eligible, all ones: always taken) are
+ * in shared memory, a run of them for every warp of the team. A histogram of
+ * the scores over 256 equal bins between the lowest and the highest narrows the
+ * place of the topk-th down to one bin; where only a part of the bin is
+ * wanted, a search over the bits of its keys finds the cut. */
+__device__ __forceinline__ void choose(const Select &p, Team t, const unsigned long long *keys, unsigned *hist, int *list) {
+    const int lane = threadIdx.x & 31;
+    const int run = ((p.k_blocks + t.warps - 1) / t.warps + 31) & ~31;
+    const int j0 = t.me * run < p.k_blocks ? t.me * run : p.k_blocks;
+    const int j1 = j0 + run < p.k_blocks ? j0 + run : p.k_blocks;
+    unsigned eligible = 0, kept = 0, x, y, top = 0, bottom = 0;
+    for (int j = j0 + lane; j < j1; j += 32) {
         const unsigned long long k = keys[j];
         eligible += k != 0ull;
-        hi = k > hi ? k : hi;
-        lo = k != 0ull && k < lo ? k : lo;
+        kept += k == ~0ull;
+        if (k != 0ull && k != ~0ull) {
+            const uint32_t f = ordered(score_of(k));
+            top = f > top ? f : top;
+            bottom = ~f > bottom ? ~f : bottom;
+        }
     }
-    eligible = __reduce_add_sync(0xffffffffu, eligible);
-    int want = p.topk < eligible ? p.topk : eligible;
+    for (int i = t.me * 32 + lane; i < kBins; i += t.warps * 32) hist[i] = 0u;
+    __syncwarp();
+    t.sum(eligible, kept, x, y);
+    t.most(top, bottom);
+    const unsigned want = (unsigned)p.topk < eligible ? (unsigned)p.topk : eligible;
     unsigned long long cut = 1ull;               /* keys above the cut are taken, equal ones from the lowest index */
     if (want < eligible) {
+        unsigned long long lo = 1ull, hi = ~0ull;          /* lo is reached by enough keys; the answer is not above hi */
+        const float low = unordered(~bottom), range = unordered(top) - low;
+        if (want <= kept) {
+            lo = ~0ull;                                    /* the places are taken already */
+        } else if (range > 0.0f && range < 1e30f) {
+            const float per = (float)kBins / range;
+            for (int j = j0 + lane; j < j1; j += 32) {
+                const unsigned long long k = keys[j];
+                if (k != 0ull && k != ~0ull) atomicAdd(hist + bin_of(score_of(k), low, per), 1u);
+            }
+            t.sync();
+            __syncwarp();
+            /* Scores in the bins above mine, eight bins a lane from the top. */
+            unsigned n[8], mine = 0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long a = __shfl_xor_sync(0xffffffffu, hi, o), b = __shfl_xor_sync(0xffffffffu, lo, o);
-            hi = a > hi ? a : hi;
-            lo = b < lo ? b : lo;
+            for (int i = 0; i < 8; i++) {
+                n[i] = hist[kBins - 1 - (lane * 8 + i)];
+                mine += n[i];
+            }
+            unsigned above = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned v = __shfl_up_sync(0xffffffffu, above, o);
+                if (lane >= o) above += v;
+            }
+            above -= mine;
+            const unsigned left = want - kept;             /* places for scores; one lane holds the bin of the last */
+            int bin = -1;
+            unsigned in_bin = 0, take = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (above < left && above + n[i] >= left) {
+                    bin = kBins - 1 - (lane * 8 + i);
+                    in_bin = n[i];
+                    take = left - above;
+                }
+                above += n[i];
+            }
+            const int src = __ffs(__ballot_sync(0xffffffffu, bin >= 0)) - 1;
+            bin = __shfl_sync(0xffffffffu, bin, src);
+            in_bin = __shfl_sync(0xffffffffu, in_bin, src);
+            take = __shfl_sync(0xffffffffu, take, src);
+            /* The keys of that bin span [lo, hi]. */
+            unsigned long long a = 0ull, b = ~0ull;
+            for (int j = j0 + lane; j < j1; j += 32) {
+                const unsigned long long k = keys[j];
+                if (k != 0ull && k != ~0ull && bin_of(score_of(k), low, per) == bin) {
+                    a = k > a ? k : a;
+                    b = k < b ? k : b;
+                }
+            }
+            t.span(b, a);
+            lo = b;
+            hi = take == in_bin ? b : a;
         }
-        /* The largest value that at least `want` keys reach: lo is reached by all, and the answer is not above hi. */
-        while (lo < hi) {
-            const unsigned long long mid = hi - ((hi - lo) >> 1);        /* lo < mid <= hi */
-            int n = 0;
-            for (int j = lane; j < p.k_blocks; j += 32) n += keys[j] >= mid;
-            n = __reduce_add_sync(0xffffffffu, n);
-            if (n >= want)
-                lo = mid;
-            else
-                hi = mid - 1ull;
-            if (n == want) break;
+        while (lo < hi) {                                  /* three thresholds a step: two bits */
+            const unsigned long long q = (hi - lo) / 4 + 1;     /* lo < t1 <= t2 <= t3 <= hi */
+            const unsigned long long t1 = lo + q, t2 = hi - t1 < q ? hi : t1 + q, t3 = hi - t2 < q ? hi : t2 + q;
+            unsigned n12 = 0, n3 = 0;
+            for (int j = j0 + lane; j < j1; j += 32) {
+                const unsigned long long k = keys[j];
+                n12 += (unsigned)(k >= t1) + ((unsigned)(k >= t2) << 16);
+                n3 += k >= t3;
+            }
+            t.sum(n12, n3, x, y);
+            const unsigned n1 = n12 & 0xffffu, n2 = n12 >> 16;
+            if (n3 >= want) {
+                lo = t3;
+                if (n3 == want) break;
+            } else if (n2 >= want) {
+                lo = t2;
+                hi = t3 - 1ull;
+                if (n2 == want) break;
+            } else if (n1 >= want) {
+                lo = t1;
+                hi = t2 - 1ull;
+                if (n1 == want) break;
+            } else {
+                hi = t1 - 1ull;
+            }
         }
         cut = lo;
     }
-    int above = 0;
-    for (int j = lane; j < p.k_blocks; j += 32) above += keys[j] > cut;
-    above = __reduce_add_sync(0xffffffffu, above);
-    int equal_left = want - above;               /* of the keys equal to the cut */
-    int done = 0;
-    for (int j0 = 0; j0 < p.k_blocks && done < want; j0 += 32) {
-        const unsigned long long k = j0 + lane < p.k_blocks ? keys[j0 + lane] : 0ull;
-        const unsigned eq = __ballot_sync(0xffffffffu, k != 0ull && k == cut);
-        const unsigned before = (1u << lane) - 1u;
-        const bool take = k != 0ull && (k > cut || (k == cut && __popc(eq & before) < equal_left));
+    unsigned above = 0, equal = 0, above_before, equal_before;
+    for (int j = j0 + lane; j < j1; j += 32) {
+        const unsigned long long k = keys[j];
+        above += k > cut;
+        equal += k == cut;
+    }
+    t.sum(above, equal, above_before, equal_before);
+    const unsigned equal_taken = want - above;   /* of the keys equal to the cut */
+    unsigned done = above_before + (equal_before < equal_taken ? equal_before : equal_taken);
+    unsigned equal_left = equal_before < equal_taken ? equal_taken - equal_before : 0u;
+    const unsigned before = (1u << lane) - 1u;
+    for (int j = j0; j < j1; j += 32) {
+        const unsigned long long k = j + lane < j1 ? keys[j + lane] : 0ull;
+        const unsigned eq = __ballot_sync(0xffffffffu, k == cut);
+        const bool take = k > cut || (k == cut && __popc(eq & before) < equal_left);
         const unsigned m = __ballot_sync(0xffffffffu, take);
-        if (take) list[done + __popc(m & before)] = j0 + lane;
+        if (take) list[done + __popc(m & before)] = j + lane;
         done += __popc(m);
         equal_left -= __popc(eq) < equal_left ? __popc(eq) : equal_left;
     }
-    for (int i = want + lane; i < p.topk; i += 32) list[i] = -1;
+    for (unsigned i = want + t.me * 32 + lane; i < (unsigned)p.topk; i += t.warps * 32) list[i] = -1;
 }
 
-template <bool VEC>
-__global__ void __launch_bounds__(kSelThreads)
+template <int HD>
+__global__ void __launch_bounds__(kSelThreads, 2)
 k_block_select(const __grid_constant__ Select p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    extern __shared__ unsigned long long keys[];         /* [rows][k_blocks] */
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    __shared__ unsigned team_counts[kSelWarps][4 * kSelWarps];
+    __shared__ unsigned team_hist[kSelWarps][kBins];
+    /* The rows as operand fragments [tile][product][lane], then [own_rows][k_blocks] keys. */
+    double *qf = reinterpret_cast<double *>(smem_raw);
+    const int tiles = p.rows > 8 ? 2 : 1;
+    unsigned long long *keys = reinterpret_cast<unsigned long long *>(qf + (size_t)tiles * p.steps * 32);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = p.ctas > 1 ? (int)sm100::cluster_cta_rank() : 0;
     const int g = blockIdx.y;
-    const long long r0 = (long long)blockIdx.x * p.rows;
+    const long long r0 = (long long)(blockIdx.x / (unsigned)p.ctas) * p.rows;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    int qb, head;
-    const int mine = lane >> 2;                          /* row of the score tile this lane feeds and receives */
-    const bool live = mine < p.rows && row_of(p, g, r0 + mine, &qb, &head);
-    const float *qrow = live ? p.qm + ((size_t)qb * p.heads + head) * p.head_dim : nullptr;
-    for (int j0 = warp * 8; j0 < p.k_blocks; j0 += (kSelThreads / 32) * 8) {
-        const int jb = j0 + mine;
-        const float *krow = jb < p.k_blocks ? p.km + ((size_t)jb * p.kv_heads + g) * p.head_dim : nullptr;
-        double d[2];
-        score_tile<VEC>(p, qrow, krow, lane, d);
+    int qb = 0, head = 0;
+    /* Four consecutive dimensions of a row at a time: products 4 g .. 4 g + 3 of lane 4 (row mod 8) + quarter. */
+    const int quads = p.steps;                       /* per row */
+    for (int i = threadIdx.x; i < tiles * 8 * quads; i += kSelThreads) {
+        const int row = i / quads, qd = i - row * quads, e = qd * 4;
+        const bool ok = row < p.rows && row_of(p, g, r0 + row, &qb, &head);
+        const float *src = p.qm + ((size_t)qb * p.heads + head) * p.head_dim + e;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (HD > 0) {
+            if (ok) {
+                const float4 f = __ldg(reinterpret_cast<const float4 *>(src));
+                v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (ok && e + k < p.head_dim) v[k] = __ldg(src + k);
+        }
+        double *dst = qf + (size_t)((row >> 3) * p.steps + (qd & ~3)) * 32 + (row & 7) * 4 + (qd & 3);
+#pragma unroll
+        for (int k = 0; k < 4; k++) dst[k * 32] = (double)v[k];
+    }
+    if (p.ctas > 1) sm100::cluster_sync_all();           /* every CTA has started: its shared memory may be written */
+    else __syncthreads();
+    const int b0 = rank * p.slice, b1 = b0 + p.slice < p.k_blocks ? b0 + p.slice : p.k_blocks;
+    for (int j0 = b0 + warp * 8; j0 < b1; j0 += kSelWarps * 8) {
+        const int jb = j0 + (lane >> 2);
+        double d[2][2];
+        score_tile<HD>(p, qf, jb < b1 ? p.km + ((size_t)jb * p.kv_heads + g) * p.head_dim : nullptr, lane, tiles, d);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int j = j0 + (lane & 3) * 2 + i;
-            if (mine < p.rows && j < p.k_blocks) {
-                const bool ok = !p.counts || __ldg(p.counts + j) > 0;
-                const bool kept = j < p.keep_first || j >= p.k_blocks - p.keep_last;
-                keys[(size_t)mine * p.k_blocks + j] = !ok ? 0ull : (kept ? ~0ull : key_of(d[i]));
+            if (j >= b1) continue;
+            const bool ok = !p.counts || __ldg(p.counts + j) > 0;
+            const bool kept = j < p.keep_first || j >= p.k_blocks - p.keep_last;
+            for (int m = 0; m < tiles; m++) {
+                const int row = m * 8 + (lane >> 2);
+                if (row >= p.rows) continue;
+                const unsigned long long key = !ok ? 0ull : (kept ? ~0ull : key_of(d[m][i]));
+                /* Row r is chosen by CTA r mod ctas, as its row r / ctas. */
+                unsigned long long *dst = keys + (size_t)(row / p.ctas) * p.k_blocks + j;
+                if (p.ctas == 1)
+                    *dst = key;
+                else
+                    asm volatile("st.shared::cluster.u64 [%0], %1;"
+                                 ::"r"(sm100::map_to_cta(sm100::smem_u32(dst), row % p.ctas)), "l"(key) : "memory");
             }
         }
     }
-    __syncthreads();
-    for (int r = warp; r < p.rows; r += kSelThreads / 32)
-        if (row_of(p, g, r0 + r, &qb, &head))
-            choose(p, keys + (size_t)r * p.k_blocks, p.list + ((size_t)head * p.q_blocks + qb) * p.topk, lane);
+    __syncwarp();
+    if (p.ctas > 1) sm100::cluster_sync_all();
+    else __syncthreads();
+    Team t = {warp % p.team, p.team, 1 + warp / p.team, team_counts[warp / p.team], 0u};
+    for (int r = warp / p.team; r < p.own_rows; r += kSelWarps / p.team) {
+        const int row = r * p.ctas + rank;
+        if (row < p.rows && row_of(p, g, r0 + row, &qb, &head))
+            choose(p, t, keys + (size_t)r * p.k_blocks, team_hist[warp / p.team], p.list + ((size_t)head * p.q_blocks + qb) * p.topk);
+        __syncwarp();
+        t.sync();
+    }
 }
 
 static int g_select_ready = 0;
@@ -316,10 +530,14 @@ extern "C" int iris_b200_block_select(int *list, const float *q_means, const flo
     if ((long long)keep_first + keep_last > topk) return bad(op, "more blocks to keep than the list holds");
     if (kv_heads > 65535) return bad(op, "too many key heads");
     if (k_blocks > kMaxBlocks) {
-        set_error(IRIS_B200_EUNSUPPORTED, op, "more than 24576 key blocks");
+        set_error(IRIS_B200_EUNSUPPORTED, op, "more than 23552 key blocks");
         return IRIS_B200_EUNSUPPORTED;
     }
     if (q_blocks > 0 && (!list || !q_means || (k_blocks > 0 && !k_means))) return bad(op, "bad argument");
+    if (head_dim > kMaxHeadDim) {
+        set_error(IRIS_B200_EUNSUPPORTED, op, "head_dim above 512");
+        return IRIS_B200_EUNSUPPORTED;
+    }
     if (!require_device(op)) return IRIS_B200_ENODEV;
     if (q_blocks == 0) return IRIS_B200_OK;
     Select p = {};
@@ -336,22 +554,48 @@ extern "C" int iris_b200_block_select(int *list, const float *q_means, const flo
     p.topk = topk;
     p.keep_first = keep_first < k_blocks ? keep_first : k_blocks;
     p.keep_last = keep_last < k_blocks ? keep_last : k_blocks;
-    p.rows = kSelRows;
-    while (p.rows > 1 && p.rows * k_blocks > kMaxBlocks) p.rows--;
-    const bool vec = head_dim % 16 == 0 && aligned16(q_means) && aligned16(k_means);
-    const size_t smem = (size_t)p.rows * k_blocks * 8;
+    p.steps = (head_dim + 15) / 16 * 4;
+    /* Rows of a cluster: as many as there are, up to two score tiles, and as
+     * the keys of fit in shared memory. The blocks are cut over a cluster while
+     * that leaves SMs idle otherwise (two CTAs per SM), down to one tile of
+     * eight blocks per warp. */
+    const long long rows = (long long)q_blocks * p.group;
+    p.rows = rows < kSelRows ? (int)rows : kSelRows;
+    auto tiles_of = [&] { return (rows + p.rows - 1) / p.rows; };
+    p.ctas = 1;
+    while (p.ctas < kMaxCtas && tiles_of() * kv_heads * p.ctas * 2 <= 2LL * g.sm_count && k_blocks >= p.ctas * 2 * kSelWarps * 8)
+        p.ctas *= 2;
+    auto smem_of = [&] {
+        p.own_rows = (p.rows + p.ctas - 1) / p.ctas;
+        return (size_t)(p.rows > 8 ? 2 : 1) * p.steps * 256 + (size_t)p.own_rows * k_blocks * 8;
+    };
+    while (p.rows > 1 && smem_of() > kSelSmem) p.rows--;
+    const size_t smem = smem_of();
+    p.slice = ((k_blocks + p.ctas - 1) / p.ctas + 7) / 8 * 8;
+    p.team = p.own_rows >= kSelWarps ? 1 : p.own_rows > 2 ? 2 : p.own_rows > 1 ? 4 : 8;
     if (!g_select_ready) {
-        if (!cuda_ok(cudaFuncSetAttribute(k_block_select<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBlocks * 8), op) ||
-            !cuda_ok(cudaFuncSetAttribute(k_block_select<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBlocks * 8), op))
+        if (!cuda_ok(cudaFuncSetAttribute(k_block_select<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem), op) ||
+            !cuda_ok(cudaFuncSetAttribute(k_block_select<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem), op) ||
+            !cuda_ok(cudaFuncSetAttribute(k_block_select<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem), op))
             return IRIS_B200_ECUDA;
         g_select_ready = 1;
     }
-    const long long rows = (long long)q_blocks * p.group, tiles = (rows + p.rows - 1) / p.rows;
-    if (tiles > INT_MAX) return bad(op, "too many query blocks");
+    const long long clusters = tiles_of();
+    if (clusters * p.ctas > INT_MAX) return bad(op, "too many query blocks");
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    configure(&cfg, &attr, dim3((unsigned)tiles, (unsigned)kv_heads), kSelThreads, smem);
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, vec ? k_block_select<true> : k_block_select<false>, p);
+    cudaLaunchAttribute attr[2];
+    configure(&cfg, attr, dim3((unsigned)(clusters * p.ctas), (unsigned)kv_heads), kSelThreads, smem);
+    if (p.ctas > 1) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = (unsigned)p.ctas;
+        attr[1].val.clusterDim.y = 1;
+        attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+    }
+    const bool aligned = aligned16(k_means) && aligned16(q_means);
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, aligned && head_dim == 128  ? k_block_select<128>
+                                                     : aligned && head_dim == 64 ? k_block_select<64>
+                                                                                 : k_block_select<0>, p);
     g.launches++;
     return cuda_ok(err, op) ? IRIS_B200_OK : IRIS_B200_ECUDA;
 }

@@ -114,7 +114,8 @@ def test_block_means_and_select_refusals(lib):
     for kw in (dict(lst=None), dict(qm=None), dict(km=None), dict(nq=-1), dict(nk=-1), dict(heads=0), dict(kv=0), dict(kv=3),
                dict(hd=0), dict(topk=0), dict(first=-1), dict(last=-1), dict(first=2, last=1)):
         refused(lib, EINVAL, select(**kw))
-    refused(lib, EUNSUPPORTED, select(nk=24577))
+    refused(lib, EUNSUPPORTED, select(nk=23553))
+    refused(lib, EUNSUPPORTED, select(hd=513))
 
 
 def test_attention_blocks_refusals(lib):

@@ -266,7 +266,9 @@ def run_select(lib, qm, km, counts, topk, first, last):
 @pytest.mark.parametrize("nq,nk,heads,kv,hd,topk,first,last", [
     (1, 1, 1, 1, 128, 1, 0, 0), (1, 5, 2, 1, 128, 9, 1, 1), (9, 33, 6, 3, 128, 7, 2, 0), (5, 264, 3, 3, 128, 40, 8, 3),
     (17, 31, 4, 4, 64, 31, 0, 0), (3, 40, 2, 2, 24, 5, 0, 5), (3, 40, 2, 1, 7, 5, 0, 2), (2, 3500, 2, 2, 128, 64, 1, 2),
-    (2, 6000, 5, 1, 16, 100, 0, 0), (1, 24576, 1, 1, 16, 17, 0, 0), (4, 2, 2, 2, 128, 6, 3, 3)])
+    (2, 6000, 5, 1, 16, 100, 0, 0), (1, 23552, 1, 1, 16, 17, 0, 0), (4, 2, 2, 2, 128, 6, 3, 3),
+    (1, 130, 4, 4, 128, 30, 0, 0), (1, 515, 8, 2, 128, 64, 1, 2), (2, 1030, 16, 2, 128, 1, 0, 0), (3, 23552, 1, 1, 24, 300, 0, 1),
+    (1, 600, 5, 1, 128, 599, 0, 0), (21, 300, 3, 1, 512, 20, 0, 0)])
 def test_block_select(lib, nq, nk, heads, kv, hd, topk, first, last):
     qm, km = randn(nk, nq, heads, hd), randn(nk + 1, nk, kv, hd)
     gen = torch.Generator().manual_seed(nq)
