@@ -321,7 +321,8 @@ def _plain_attention(s):
 
 def _own(s):
     case, lib, op = s["case"], s["lib"], s["case"]["op"]
-    lib.iris_b200_use_stream(torch.cuda.current_stream().cuda_stream)
+    # 1 is CUDA's handle of the default stream; 0 would mean the library's own.
+    lib.iris_b200_use_stream(torch.cuda.current_stream().cuda_stream or 1)
     if op == "prologue":
         x, hq, hk = s["x"].data_ptr(), case["heads"], case["kv_heads"]
         wq, wk = (s["wq"].data_ptr(), s["wk"].data_ptr()) if case["norm"] else (None, None)
