@@ -18,7 +18,7 @@
  *   A key tile is 128 rows made of 128 / k_block listed blocks (or a piece of
  *   a longer block), each its own TMA box, so blocks may lie anywhere. The
  *   producer warp reads the list 32 entries at a time, skips what names no
- *   block, and publishes with every tile one bit per key: zero for rows behind
+ *   block or holds no valid key, and publishes with every tile one bit per key: zero for rows behind
  *   seq_k, masked rows and the rows of a last tile that no block filled. Their
  *   scores become -inf whatever K holds; their V rows are cleared in shared
  *   memory before the MMA, since a zero probability does not cancel a NaN.
@@ -109,6 +109,25 @@ struct Params {
     unsigned long long wait_ns;
 };
 
+/* The bounded wait of the dense kernel, except that it first looks at the clock
+ * after 64 tries: reading it takes about a thousand cycles, which a wait that is
+ * nearly over should not pay (16 896 rows x 32 heads over 64 blocks: 1210 us
+ * with the clock read on entry, 1060 us so). */
+__device__ __forceinline__ bool wait_bar(const Ctx &c, int idx, uint32_t parity, int site) {
+    const uint32_t bar = c.bars + idx * 8;
+    unsigned long long t0 = 0;
+    for (uint32_t spin = 1;; spin++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (spin % 64u != 0) continue;
+        if (*c.abort_flag) return false;
+        if (t0 == 0) t0 = global_ns();
+        if (global_ns() - t0 > c.wait_ns || spin > (1u << 26)) {
+            give_up(c, site, parity);
+            return false;
+        }
+    }
+}
+
 struct Tile {
     int head, q0, rows;                 /* first row and rows that exist */
     const int *list;
@@ -116,11 +135,9 @@ struct Tile {
 };
 __device__ __forceinline__ Tile tile_of(const Params &p, int rank) {
     Tile t;
-    const unsigned item = blockIdx.x / (unsigned)p.parts;
-    const unsigned per_head = (unsigned)p.q_blocks * (unsigned)p.tiles;
-    t.head = (int)(item / per_head);
-    const unsigned in_head = item - (unsigned)t.head * per_head;
-    const int qb = (int)(in_head / (unsigned)p.tiles), in_block = (int)(in_head - (unsigned)qb * p.tiles) * kTile;
+    t.head = (int)blockIdx.y;
+    const int in_head = p.parts > 1 ? (int)(blockIdx.x / (unsigned)p.parts) : (int)blockIdx.x;
+    const int qb = p.tiles > 1 ? in_head / p.tiles : in_head, in_block = (in_head - qb * p.tiles) * kTile;
     t.q0 = qb * p.q_block + in_block;
     int rows = p.q_block - in_block < kTile ? p.q_block - in_block : kTile;
     if (p.seq_q - t.q0 < rows) rows = p.seq_q - t.q0;
@@ -137,50 +154,42 @@ __device__ __forceinline__ void producer(const Ctx &c, const Params &p, const Ti
     const int qcol = t.head * kHeadDim, kcol = (t.head / p.group) * kHeadDim;
     int j = 0;                          /* tiles published */
     int loads_k = 0, loads_v = 0;       /* tiles whose K / V copies were started */
+    /* Q and the first entries of the list are on their way before anything else. */
+    int entry = t.e0 + lane < t.e1 ? __ldg(t.list + t.e0 + lane) : -1;
+    if (lane == 0 && t.e0 < t.e1) {
+        mbar_expect_tx(c.bars + BAR_Q_FULL * 8, kTileBytes);
+        for (int half = 0; half < 2; half++)
+            tma_load_2d(smem + kSmemQ + half * kHalfBytes, mq, qcol + half * 64, t.q0, c.bars + BAR_Q_FULL * 8);
+    }
+    __syncwarp();
     int filled = 0;                     /* boxes of the tile being put together; lane u holds the first row of box u */
     int row_of_unit = 0;
+    uint32_t key_bits = 0;              /* lane w: valid keys [32 w, 32 w + 32) of the tile */
     bool ok = true;
 
     /* Publish (and load) the tile at hand; the end of the list when it is empty. */
     auto emit = [&]() -> bool {
         const int n = filled;
-        /* The valid keys. Key 32 w + lane of the tile lies in box key / unit. */
-        uint32_t bits[4];
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const int key = 32 * w + lane, u = key / p.unit;
-            const int row = __shfl_sync(0xffffffffu, row_of_unit, u) + (key - u * p.unit);
-            bool valid = u < n && row < p.seq_k;
-            if (valid && p.key_mask) valid = __ldg(p.key_mask + row) != 0;
-            bits[w] = __ballot_sync(0xffffffffu, valid);
-        }
         const uint32_t par = (uint32_t)(j - 1) & 1u;
         /* QK(j - 1) is done: K's buffer is free, and every reader is through with the tile record of four tiles ago. */
-        if (j > 0 && !__all_sync(0xffffffffu, mbar_wait(c, BAR_K_EMPTY, par, 400))) return false;
+        if (j > 0 && !__all_sync(0xffffffffu, wait_bar(c, BAR_K_EMPTY, par, 400))) return false;
         volatile Meta *m = meta + (j & (kMetaSlots - 1));
-        if (lane == 0) {
-            for (int w = 0; w < 4; w++) m->bits[w] = bits[w];
-            m->state = n == 0 ? 0u : ((bits[0] & bits[1] & bits[2] & bits[3]) == 0xFFFFFFFFu ? 1u : 2u);
-            mbar_arrive(c.bars + (BAR_META + (j & (kMetaSlots - 1))) * 8);
-        }
+        const bool whole = __all_sync(0xffffffffu, lane >= 4 || key_bits == 0xFFFFFFFFu);
+        if (lane < 4) m->bits[lane] = key_bits;
+        key_bits = 0;
+        if (lane == 0) m->state = n == 0 ? 0u : whole ? 1u : 2u;
         __syncwarp();
+        if (lane == 0) mbar_arrive(c.bars + (BAR_META + (j & (kMetaSlots - 1))) * 8);
         if (n == 0) return true;
         const uint32_t bytes = (uint32_t)(n * p.unit * 256);
-        if (lane == 0) {
-            if (j == 0) {
-                mbar_expect_tx(c.bars + BAR_Q_FULL * 8, kTileBytes);
-                for (int half = 0; half < 2; half++)
-                    tma_load_2d(smem + kSmemQ + half * kHalfBytes, mq, qcol + half * 64, t.q0, c.bars + BAR_Q_FULL * 8);
-            }
-            mbar_expect_tx(c.bars + BAR_K_FULL * 8, bytes);
-        }
+        if (lane == 0) mbar_expect_tx(c.bars + BAR_K_FULL * 8, bytes);
         __syncwarp();
         if (lane < n)
             for (int half = 0; half < 2; half++)
                 tma_load_2d(smem + kSmemK + half * kHalfBytes + lane * p.unit * 128, mk, kcol + half * 64, row_of_unit,
                             c.bars + BAR_K_FULL * 8);
         loads_k++;
-        if (j > 0 && !__all_sync(0xffffffffu, mbar_wait(c, BAR_V_EMPTY, par, 401))) return false;
+        if (j > 0 && !__all_sync(0xffffffffu, wait_bar(c, BAR_V_EMPTY, par, 401))) return false;
         if (lane == 0) mbar_expect_tx(c.bars + BAR_V_FULL * 8, bytes);
         __syncwarp();
         if (lane < n)
@@ -194,20 +203,38 @@ __device__ __forceinline__ void producer(const Ctx &c, const Params &p, const Ti
         return true;
     };
 
+    /* One box of rows joins the tile at hand, unless the mask leaves none of them. */
+    auto add = [&](int row0) -> bool {
+        uint32_t any = 0, bits = 0;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const int key = 32 * w + lane;
+            bool valid = key < p.unit && row0 + key < p.seq_k;
+            if (valid && p.key_mask) valid = __ldg(p.key_mask + row0 + key) != 0;
+            const uint32_t b = __ballot_sync(0xffffffffu, valid);
+            any |= b;
+            /* Word of the tile that these keys belong to (two boxes of 16 keys share one). */
+            if (lane == (filled * p.unit >> 5) + w) bits = p.unit == 16 ? b << (16 * (filled & 1)) : b;
+        }
+        if (any == 0) return true;
+        if (32 * lane < kTile) key_bits |= bits;
+        if (lane == filled) row_of_unit = row0;
+        return ++filled < p.units || emit();
+    };
+
     for (int e = t.e0; ok && e < t.e1; e += 32) {
-        const int entry = e + lane < t.e1 ? __ldg(t.list + e + lane) : -1;
+        if (e > t.e0) entry = e + lane < t.e1 ? __ldg(t.list + e + lane) : -1;
         unsigned todo = __ballot_sync(0xffffffffu, entry >= 0 && entry < p.k_blocks);
         while (ok && todo) {
             const int src = __ffs(todo) - 1;
             todo &= todo - 1;
             const int row0 = __shfl_sync(0xffffffffu, entry, src) * p.k_block;     /* < seq_k */
-            for (int s = 0; ok && s < p.per_entry && row0 + s * kTile < p.seq_k; s++) {
-                if (lane == filled) row_of_unit = row0 + s * kTile;
-                if (++filled == p.units) ok = emit();
-            }
+            for (int s = 0; ok && s < p.per_entry && row0 + s * kTile < p.seq_k; s++) ok = add(row0 + s * kTile);
         }
     }
     if (ok && filled > 0) ok = emit();
+    /* (Without any block nobody else waits for Q, whose place the epilogue uses.) */
+    if (ok && j == 0 && t.e0 < t.e1) ok = __all_sync(0xffffffffu, wait_bar(c, BAR_Q_FULL, 0, 402));
     if (ok) ok = emit();
     if (*c.abort_flag) {
         /* Nobody may be consuming any more: wait (bounded by the limit again) for the copies still in flight. */
@@ -215,7 +242,7 @@ __device__ __forceinline__ void producer(const Ctx &c, const Params &p, const Ti
         auto drain = [&](int bar, int n) {
             while (n > 0 && !mbar_try_wait(c.bars + bar * 8, (uint32_t)(n - 1) & 1u) && global_ns() - t0 < c.wait_ns) {}
         };
-        drain(BAR_Q_FULL, loads_k > 0);
+        drain(BAR_Q_FULL, t.e0 < t.e1);
         drain(BAR_K_FULL, loads_k);
         drain(BAR_V_FULL, loads_v);
     }
@@ -247,7 +274,7 @@ __device__ __forceinline__ void mma_issuer(const Ctx &c, uint32_t smem, unsigned
     bool ok = true;
 
     auto wait_all = [&](int bar, uint32_t par, int site) -> bool {
-        return __all_sync(0xffffffffu, mbar_wait(c, bar, par, site));
+        return __all_sync(0xffffffffu, wait_bar(c, bar, par, site));
     };
     auto state_of = [&](int j) -> uint32_t { return meta[j & (kMetaSlots - 1)].state; };
     auto issue_qk = [&]() {
@@ -320,11 +347,11 @@ __device__ __forceinline__ RowState softmax_rows(const Ctx &c, const Params &p, 
     RowState st = {-INFINITY, 0.0f, false, true};
     for (int j = 0;; j++) {
         const int slot = j & (kMetaSlots - 1);
-        if (!(st.ok = __all_sync(0xffffffffu, mbar_wait(c, BAR_META + slot, (uint32_t)(j / kMetaSlots) & 1u, 420)))) return st;
+        if (!(st.ok = __all_sync(0xffffffffu, wait_bar(c, BAR_META + slot, (uint32_t)(j / kMetaSlots) & 1u, 420)))) return st;
         const uint32_t state = meta[slot].state;
         if (state == 0u) break;
         st.any = true;
-        if (!(st.ok = __all_sync(0xffffffffu, mbar_wait(c, BAR_S_FULL, (uint32_t)j & 1u, 421)))) return st;
+        if (!(st.ok = __all_sync(0xffffffffu, wait_bar(c, BAR_S_FULL, (uint32_t)j & 1u, 421)))) return st;
         tc_fence_after();
         if (!live) {
             /* Rows that do not exist: whatever lies in P only meets rows of O that nobody reads. */
@@ -339,7 +366,10 @@ __device__ __forceinline__ RowState softmax_rows(const Ctx &c, const Params &p, 
         tc_wait_ld();
         if (state == 2u) {
 #pragma unroll
-            for (int ch = 0; ch < 4; ch++) mask_chunk(s + ch * 32, meta[slot].bits[ch]);
+            for (int ch = 0; ch < 4; ch++) {
+                const uint32_t bits = meta[slot].bits[ch];
+                if (bits != 0xFFFFFFFFu) mask_chunk(s + ch * 32, bits);
+            }
         }
         float mx8[8];
 #pragma unroll
@@ -386,46 +416,50 @@ __device__ __forceinline__ RowState softmax_rows(const Ctx &c, const Params &p, 
         st.l += (sum4[0] + sum4[2]) + (sum4[1] + sum4[3]);
     }
     if (st.any) {
-        st.ok = __all_sync(0xffffffffu, mbar_wait(c, BAR_O_DONE, 0, 422));
+        st.ok = __all_sync(0xffffffffu, wait_bar(c, BAR_O_DONE, 0, 422));
         tc_fence_after();
     }
     return st;
 }
 
-/* O times f -> bf16 rows, through 4 KB of staging per warp (32 rows x 128
- * bytes, 16-byte chunks swizzled by the row): a thread owns a row, memory wants
+/* O times f -> bf16 rows, through 8 KB of staging per warp (two halves of 32
+ * rows x 128 bytes, 16-byte chunks swizzled by the row): a thread owns a row, memory wants
  * eight threads per 128 bytes of it. */
 __device__ __forceinline__ void store_rows(const Params &p, const Tile &t, uint32_t tmem, float f, bool any, unsigned char *stage) {
     const int row = threadIdx.x & 127, lane = threadIdx.x & 31, row0 = row & ~31;
     if (row0 >= t.rows) return;
     const uint32_t tO = tmem + ((uint32_t)row0 << 16) + 128;
-    unsigned char *sw = stage + (row0 >> 5) * 4096;
+    unsigned char *sw = stage + (row0 >> 5) * 8192;
     uint16_t *out = p.out + (size_t)(t.q0 + row0) * p.ldo + (size_t)t.head * kHeadDim;
+    uint32_t o[128];
+    if (any) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) tmem_ld32(tO + q * 32, o + q * 32);
+        tc_wait_ld();
+    }
 #pragma unroll
     for (int half = 0; half < 2; half++) {
-        uint32_t o[64];
-        if (any) {
-            tmem_ld32(tO + half * 64, o);
-            tmem_ld32(tO + half * 64 + 32, o + 32);
-            tc_wait_ld();
-        }
 #pragma unroll
         for (int ch = 0; ch < 8; ch++) {
             uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                w[e] = any && f != 0.0f ? cvt_bf16x2(__uint_as_float(o[8 * ch + 2 * e]) * f, __uint_as_float(o[8 * ch + 2 * e + 1]) * f) : 0u;
-            *reinterpret_cast<uint4 *>(sw + lane * 128 + ((ch ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int e = 0; e < 4; e++) {
+                const float a = __uint_as_float(o[64 * half + 8 * ch + 2 * e]), b = __uint_as_float(o[64 * half + 8 * ch + 2 * e + 1]);
+                w[e] = any && f != 0.0f ? cvt_bf16x2(a * f, b * f) : 0u;
+            }
+            *reinterpret_cast<uint4 *>(sw + half * 4096 + lane * 128 + ((ch ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        __syncwarp();
-        const int ch = lane & 7;
+    }
+    __syncwarp();
+    const int ch = lane & 7;
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             const int r = k * 4 + (lane >> 3);
-            const uint4 v = *reinterpret_cast<const uint4 *>(sw + r * 128 + ((ch ^ (r & 7)) << 4));
+            const uint4 v = *reinterpret_cast<const uint4 *>(sw + half * 4096 + r * 128 + ((ch ^ (r & 7)) << 4));
             if (row0 + r < t.rows) *reinterpret_cast<uint4 *>(out + (size_t)r * p.ldo + half * 64 + ch * 8) = v;
         }
-        __syncwarp();
     }
 }
 
@@ -459,25 +493,34 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
     c.wait_ns = p.wait_ns;
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + kSmemBar + kOffTmemPtr);
     volatile Meta *meta = reinterpret_cast<volatile Meta *>(smem_gen + kSmemBar + kOffMeta);
-    if (threadIdx.x == 0) {
-        for (int b = 0; b < BAR_COUNT; b++) mbar_init(c.bars + b * 8, b == BAR_P_FULL || b == BAR_P_FULL + 1 ? 128 : 1);
-        *c.abort_flag = 0u;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    if (warp == 5) {
-        __syncwarp();
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem + kSmemBar + kOffTmemPtr), "r"(256u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    /* Launched with programmatic stream serialisation: nothing below may start before the kernel ahead is complete. */
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const Tile t = tile_of(p, rank);
+    /* The producer sets up the barriers and starts at once; it only tells the
+     * other warps, which wait here for the barriers and the tensor memory. The
+     * launch is stream-serialised by program: nothing may be read or written
+     * before the kernel ahead is complete, which the producer waits for and
+     * everything else follows from its loads. */
+    uint32_t tmem = 0;
+    if (warp == 4) {
+        if (lane == 0) {
+            for (int b = 0; b < BAR_COUNT; b++) mbar_init(c.bars + b * 8, b == BAR_P_FULL || b == BAR_P_FULL + 1 ? 128 : 1);
+            *c.abort_flag = 0u;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        asm volatile("barrier.cta.arrive.aligned 1, %0;" ::"n"(kThreads) : "memory");
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+    } else {
+        if (warp == 5) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                         ::"r"(smem + kSmemBar + kOffTmemPtr), "r"(256u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+            tc_fence_before();
+        }
+        asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(kThreads) : "memory");
+        tc_fence_after();
+        tmem = *tmem_slot;
+    }
 
     RowState st = {-INFINITY, 0.0f, false, true};
     if (warp < 4) {
@@ -621,7 +664,7 @@ int launch_attention_blocks_sm100(const BlockAttnArgs &a) {
         !make_tensor_map(&tmv, a.v, a.seq_k, a.kv_heads * kHeadDim, a.ldv, p.unit))
         return IRIS_B200_ECUDA;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(items * p.parts));
+    cfg.gridDim = dim3((unsigned)(a.q_blocks * p.tiles * p.parts), (unsigned)a.heads);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kSmemBytes;
     cfg.stream = g.stream;
