@@ -4,7 +4,7 @@
  *
  * k_block_means reads every element once and is bound by HBM. A CTA owns one
  * block of rows and 256 columns, 32 lanes x 16 bytes; its eight warps take
- * every eighth row. A thread adds up to sixteen rows in fp32 and joins these
+ * every eighth row. A thread adds up to eight rows in fp32 and joins these
  * partial sums, and then the warps', in fp64, so that a mean is off by no more
  * than the rounding of a few sixteen-row sums.
  *
@@ -35,11 +35,11 @@ namespace block_select {
 
 static constexpr int kMeanThreads = 256;
 static constexpr int kMeanCols = 256;            /* columns of a CTA */
-static constexpr int kMeanRun = 16;              /* rows of a thread summed in fp32 */
+static constexpr int kMeanRun = 8;               /* rows of a thread in flight, and summed in fp32 */
 
 /* VEC: 16-byte loads (head_dim and strides multiples of 8, aligned base). */
 template <bool VEC>
-__global__ void __launch_bounds__(kMeanThreads)
+__global__ void __launch_bounds__(kMeanThreads, 4)
 k_block_means(float *__restrict__ means, int *__restrict__ counts, const uint16_t *__restrict__ x, int ldx, int seq,
               int width, int block, const int *__restrict__ row_mask) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -55,38 +55,36 @@ k_block_means(float *__restrict__ means, int *__restrict__ counts, const uint16_
     for (int i = 0; i < 8; i++) acc[i] = 0.0;
     int n = 0;
     for (int rb = warp; rb < rows; rb += 8 * kMeanRun) {
+        /* Which of the run's rows count (bit i: row rb + 8 i), then all their loads at once. */
+        const int mine = rb + 8 * lane;
+        const bool counts_mine = lane < kMeanRun && mine < rows && (!row_mask || __ldg(row_mask + r0 + mine) != 0);
+        const unsigned ok = __ballot_sync(0xffffffffu, counts_mine);
+        n += __popc(ok);
+        uint4 v[kMeanRun];
+#pragma unroll
+        for (int i = 0; i < kMeanRun; i++) {
+            v[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (!((ok >> i) & 1u)) continue;
+            const uint16_t *src = x + (size_t)(r0 + rb + 8 * i) * ldx + c0;
+            if (VEC) {
+                if (c0 < width) v[i] = __ldg(reinterpret_cast<const uint4 *>(src));
+            } else {
+                uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (c0 + e < width) w[e >> 1] |= (uint32_t)src[e] << (16 * (e & 1));
+                v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
         float s[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) s[i] = 0.0f;
 #pragma unroll
-        for (int b = 0; b < kMeanRun; b += 8) {
-            uint4 v[8];
-            bool ok[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int r = rb + (b + i) * 8;
-                ok[i] = r < rows && (!row_mask || __ldg(row_mask + r0 + r) != 0);
-                v[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (!ok[i]) continue;
-                const uint16_t *src = x + (size_t)(r0 + r) * ldx + c0;
-                if (VEC) {
-                    if (c0 < width) v[i] = __ldg(reinterpret_cast<const uint4 *>(src));
-                } else {
-                    uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (c0 + e < width) w[e >> 1] |= (uint32_t)src[e] << (16 * (e & 1));
-                    v[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                n += ok[i];
-                s[0] += bf_lo(v[i].x); s[1] += bf_hi(v[i].x);
-                s[2] += bf_lo(v[i].y); s[3] += bf_hi(v[i].y);
-                s[4] += bf_lo(v[i].z); s[5] += bf_hi(v[i].z);
-                s[6] += bf_lo(v[i].w); s[7] += bf_hi(v[i].w);
-            }
+        for (int i = 0; i < kMeanRun; i++) {
+            s[0] += bf_lo(v[i].x); s[1] += bf_hi(v[i].x);
+            s[2] += bf_lo(v[i].y); s[3] += bf_hi(v[i].y);
+            s[4] += bf_lo(v[i].z); s[5] += bf_hi(v[i].z);
+            s[6] += bf_lo(v[i].w); s[7] += bf_hi(v[i].w);
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) acc[i] += (double)s[i];
