@@ -6,7 +6,7 @@
  * block of rows and 256 columns, 32 lanes x 16 bytes; its eight warps take
  * every eighth row. A thread adds up to eight rows in fp32 and joins these
  * partial sums, and then the warps', in fp64, so that a mean is off by no more
- * than the rounding of a few sixteen-row sums.
+ * than the rounding of a few eight-row sums.
  *
  * k_block_select scores in fp64: a product of two fp32 means is exact there,
  * and a list only depends on the order of summation where two scores agree to

@@ -7,9 +7,10 @@
  * whole turns fall off by themselves, for any sign and size of p, with an
  * error of |p| 2^-65 turns; there is no range reduction and no table. Of the
  * phase the top 32 bits are used (2^-32 turns = 1.5e-9 rad): the two highest
- * give the quadrant after rounding, the rest an angle within pi / 4 on which
- * the Taylor series of sine (to a^9) and cosine (to a^10) are within 2e-9 of
- * the functions, below the rounding of fp32.
+ * give the quadrant after rounding, the rest an angle a within pi / 4 on which
+ * a + a^3 S(a^2) and 1 - a^2 / 2 + a^4 C(a^2), with quadratics S and C of least
+ * maximum error (an iteratively reweighted least-squares fit), are within
+ * 2.3e-9 of sine and cosine, below the rounding of fp32.
  *
  * k_rope_tables writes 8 bytes per pair and is bound by those stores.
  *
@@ -34,47 +35,52 @@ namespace rope_axes {
 static constexpr int kThreads = 256;
 static constexpr int kInFlight = 4;          /* units of a lane group loaded before the first is used */
 static constexpr int kBlocksPerSM = 4;
+static constexpr int kTableRows = 4;         /* rows of a thread of k_rope_tables whose positions are in flight */
 static constexpr int kMaxPairs = IRIS_B200_ROPE_MAX_PAIRS;
 
+/* F_j as two words of which the lower counts as signed: F_j = hi 2^32 + lo modulo 2^64. */
+struct Turn {
+    uint32_t hi;
+    int lo;
+};
 struct Plan {
     int n;                                   /* positions per row */
-    unsigned long long turn[kMaxPairs];      /* F_j */
+    Turn turn[kMaxPairs];
     unsigned char axis[kMaxPairs];
 };
 
 /* cos and sin of the phase p * turn. */
-__device__ __forceinline__ void turn_of(int p, unsigned long long turn, float &cs, float &sn) {
-    const uint32_t top = (uint32_t)(((unsigned long long)(long long)p * turn) >> 32);
-    const uint32_t quad = (top + 0x20000000u) >> 30;
-    const float a = (float)(int)(top - (quad << 30)) * 1.4629180792671596e-09f;     /* 2 pi / 2^32 */
+__device__ __forceinline__ void turn_of(int p, Turn t, float &cs, float &sn) {
+    /* Bits 32 to 63 of the phase plus an eighth of a turn: two bits of quadrant, then the angle from -pi / 4 up. */
+    const uint32_t top = (uint32_t)p * t.hi + (uint32_t)__mulhi(p, t.lo) + 0x20000000u;
+    const float a = (float)((int)(top & 0x3FFFFFFFu) - 0x20000000) * 1.4629180792671596e-09f;     /* 2 pi / 2^32 */
     const float b = a * a;
-    float s = fmaf(b, 1.0f / 362880.0f, -1.0f / 5040.0f);
-    s = fmaf(b, s, 1.0f / 120.0f);
-    s = fmaf(b, s, -1.0f / 6.0f);
+    float s = fmaf(b, -0.00019495636f, 0.008331979f);
+    s = fmaf(b, s, -0.16666651f);
     s = fmaf(a * b, s, a);
-    float c = fmaf(b, -1.0f / 3628800.0f, 1.0f / 40320.0f);
-    c = fmaf(b, c, -1.0f / 720.0f);
-    c = fmaf(b, c, 1.0f / 24.0f);
+    float c = fmaf(b, 2.4438452e-05f, -0.0013887368f);
+    c = fmaf(b, c, 0.041666646f);
     c = fmaf(b, c, -0.5f);
     c = fmaf(b, c, 1.0f);
-    const bool odd = quad & 1u;
+    const bool odd = top & 0x40000000u;
     const float x = odd ? s : c, y = odd ? c : s;
-    cs = __uint_as_float(__float_as_uint(x) ^ (((quad + 1u) & 2u) << 30));
-    sn = __uint_as_float(__float_as_uint(y) ^ ((quad & 2u) << 30));
+    /* cos: + - - + over the quadrants, sin: + + - -. */
+    cs = __uint_as_float(__float_as_uint(x) ^ ((top + 0x40000000u) & 0x80000000u));
+    sn = __uint_as_float(__float_as_uint(y) ^ (top & 0x80000000u));
 }
 
 /* ---- tables ---- */
 
 /* A thread keeps VEC consecutive pairs for all its rows. */
 template <int VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kBlocksPerSM)
 k_rope_tables(float *__restrict__ cos_out, float *__restrict__ sin_out, const int *__restrict__ pos, int seq, int half,
               const __grid_constant__ Plan plan) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int per_row = half / VEC, rows_per_block = kThreads / per_row;
     const int r = threadIdx.x / per_row, j = (threadIdx.x - r * per_row) * VEC;
     if (r >= rows_per_block) return;
-    unsigned long long turn[VEC];
+    Turn turn[VEC];
     int axis[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; i++) {
@@ -82,18 +88,32 @@ k_rope_tables(float *__restrict__ cos_out, float *__restrict__ sin_out, const in
         axis[i] = plan.axis[j + i];
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (long long row = (long long)blockIdx.x * rows_per_block + r; row < seq; row += (long long)gridDim.x * rows_per_block) {
-        const int *p = pos + row * plan.n;
-        float c[VEC], s[VEC];
+    const long long stride = (long long)gridDim.x * rows_per_block;
+    for (long long row0 = (long long)blockIdx.x * rows_per_block + r; row0 < seq; row0 += kTableRows * stride) {
+        int at[kTableRows][VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; i++) turn_of(__ldg(p + axis[i]), turn[i], c[i], s[i]);
-        float *co = cos_out + row * half + j, *so = sin_out + row * half + j;
-        if (VEC == 4) {
-            *reinterpret_cast<float4 *>(co) = make_float4(c[0], c[1 % VEC], c[2 % VEC], c[3 % VEC]);
-            *reinterpret_cast<float4 *>(so) = make_float4(s[0], s[1 % VEC], s[2 % VEC], s[3 % VEC]);
-        } else {
-            *co = c[0];
-            *so = s[0];
+        for (int k = 0; k < kTableRows; k++) {
+            const long long row = row0 + k * stride < seq ? row0 + k * stride : row0;
+            const int *p = pos + row * plan.n;
+            /* Neighbouring pairs mostly belong to one axis. */
+#pragma unroll
+            for (int i = 0; i < VEC; i++) at[k][i] = i > 0 && axis[i] == axis[i > 0 ? i - 1 : 0] ? at[k][i > 0 ? i - 1 : 0] : __ldg(p + axis[i]);
+        }
+#pragma unroll
+        for (int k = 0; k < kTableRows; k++) {
+            const long long row = row0 + k * stride;
+            if (row >= seq) break;
+            float c[VEC], s[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; i++) turn_of(at[k][i], turn[i], c[i], s[i]);
+            float *co = cos_out + row * half + j, *so = sin_out + row * half + j;
+            if (VEC == 4) {
+                __stcs(reinterpret_cast<float4 *>(co), make_float4(c[0], c[1 % VEC], c[2 % VEC], c[3 % VEC]));
+                __stcs(reinterpret_cast<float4 *>(so), make_float4(s[0], s[1 % VEC], s[2 % VEC], s[3 % VEC]));
+            } else {
+                *co = c[0];
+                *so = s[0];
+            }
         }
     }
 }
@@ -123,7 +143,7 @@ k_qk_norm_rope_axes(const __grid_constant__ Rows a, const __grid_constant__ Plan
     const int lane = threadIdx.x & 31, l = lane & (LANES - 1), grp = lane / LANES;
     /* The lane's pairs 4 l .. 4 l + 3 in memory. */
     const int d0 = SPLIT ? 4 * l : 8 * l, d1 = SPLIT ? HD / 2 + 4 * l : 8 * l + 4;
-    unsigned long long turn[PPL];
+    Turn turn[PPL];
     int axis[PPL];
 #pragma unroll
     for (int i = 0; i < PPL; i++) {
@@ -281,7 +301,9 @@ static bool plan_of(const iris_b200_rope_axes *axes, int head_dim, Plan *plan) {
     plan->n = axes->n;
     for (int j = 0; j < head_dim / 2; j++) {
         if (axes->axis[j] >= axes->n) return false;
-        plan->turn[j] = axes->turn[j];
+        const uint32_t lo = (uint32_t)axes->turn[j];
+        plan->turn[j].hi = (uint32_t)(axes->turn[j] >> 32) + (lo >> 31);
+        plan->turn[j].lo = (int)lo;
         plan->axis[j] = axes->axis[j];
     }
     return true;
@@ -365,7 +387,7 @@ extern "C" int iris_b200_rope_axes_tables(float *cos_out, float *sin_out, const 
     const bool vec = half % 4 == 0 && aligned(cos_out, 16) && aligned(sin_out, 16);
     const int rows_per_block = kThreads / (vec ? half / 4 : half);
     long long blocks = ((long long)seq + rows_per_block - 1) / rows_per_block;
-    if (blocks > (long long)g.sm_count * 8) blocks = (long long)g.sm_count * 8;
+    if (blocks > (long long)g.sm_count * kBlocksPerSM) blocks = (long long)g.sm_count * kBlocksPerSM;
     Launch l((unsigned)blocks);
     const cudaError_t err = vec ? cudaLaunchKernelEx(&l.cfg, k_rope_tables<4>, cos_out, sin_out, pos, seq, half, plan)
                                 : cudaLaunchKernelEx(&l.cfg, k_rope_tables<1>, cos_out, sin_out, pos, seq, half, plan);
