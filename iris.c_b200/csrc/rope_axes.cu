@@ -33,8 +33,7 @@ namespace iris_b200 {
 namespace rope_axes {
 
 static constexpr int kThreads = 256;
-static constexpr int kInFlight = 4;          /* units of a lane group loaded before the first is used */
-static constexpr int kBlocksPerSM = 4;
+static constexpr int kBlocksPerSM = 4;       /* of k_rope_tables */
 static constexpr int kTableRows = 4;         /* rows of a thread of k_rope_tables whose positions are in flight */
 static constexpr int kMaxPairs = IRIS_B200_ROPE_MAX_PAIRS;
 
@@ -133,13 +132,25 @@ struct Rows {
     float eps;
 };
 
+/* Units of a lane group that are loaded before the first is used, and CTAs per
+ * SM. The 8-byte accesses of the split pairing want twice as many in flight. At
+ * 16 896 x 64 heads (554 MB) without the split: 4 units and 3 CTAs 94 us, 4 and
+ * 4 107, 8 and 2 96, 6 and 3 95, 2 and 6 125. With it, at 31 005 x 36 heads (572
+ * MB): 8 and 2 94 us, 4 and 3 102, 8 and 3 103. */
+template <bool SPLIT>
+struct Shape {
+    static constexpr int kInFlight = SPLIT ? 8 : 4;
+    static constexpr int kBlocks = SPLIT ? 2 : 3;
+};
+
 template <int HD, bool SPLIT, bool NORM>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSM)
+__global__ void __launch_bounds__(kThreads, Shape<SPLIT>::kBlocks)
 k_qk_norm_rope_axes(const __grid_constant__ Rows a, const __grid_constant__ Plan plan) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int LANES = HD / 8;                   /* lanes of a unit */
     constexpr int GROUPS = 32 / LANES;              /* units a warp works on at a time */
     constexpr int PPL = HD / 64;                    /* pairs whose sine and cosine a lane works out */
+    constexpr int FLIGHT = Shape<SPLIT>::kInFlight;
     const int lane = threadIdx.x & 31, l = lane & (LANES - 1), grp = lane / LANES;
     /* The lane's pairs 4 l .. 4 l + 3 in memory. */
     const int d0 = SPLIT ? 4 * l : 8 * l, d1 = SPLIT ? HD / 2 + 4 * l : 8 * l + 4;
@@ -157,6 +168,31 @@ k_qk_norm_rope_axes(const __grid_constant__ Rows a, const __grid_constant__ Plan
         const int row = (int)(item / a.chunks);
         const int u0 = (int)(item - (long long)row * a.chunks) * a.chunk;     /* first head, Q heads before K heads */
         const int u1 = u0 + a.chunk;
+        int part = u0 < a.heads[0] ? 0 : 1;
+        int h = part ? u0 - a.heads[0] : u0;
+        int h1 = part ? u1 - a.heads[0] : u1;
+        if (h1 > a.heads[part]) h1 = a.heads[part];
+        uint2 va[FLIGHT], vb[FLIGHT];
+        auto load = [&]() {
+            const uint16_t *in = a.in[part] + (size_t)row * a.ldi;
+#pragma unroll
+            for (int i = 0; i < FLIGHT; i++) {
+                const int hh = h + i * GROUPS + grp;
+                va[i] = vb[i] = make_uint2(0u, 0u);
+                if (hh < h1) {
+                    const uint16_t *src = in + hh * HD;
+                    if (SPLIT) {
+                        va[i] = *reinterpret_cast<const uint2 *>(src + d0);
+                        vb[i] = *reinterpret_cast<const uint2 *>(src + d1);
+                    } else {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(src + d0);
+                        va[i] = make_uint2(v.x, v.y);
+                        vb[i] = make_uint2(v.z, v.w);
+                    }
+                }
+            }
+        };
+        load();                         /* under the way to the row's angles */
         float cs[4], sn[4];
         {
             float c[PPL], s[PPL];
@@ -169,11 +205,7 @@ k_qk_norm_rope_axes(const __grid_constant__ Rows a, const __grid_constant__ Plan
                 sn[i] = __shfl_sync(0xffffffffu, s[i % PPL], src);
             }
         }
-#pragma unroll
-        for (int part = 0; part < 2; part++) {
-            const int base = part ? a.heads[0] : 0;
-            const int h0 = (u0 > base ? u0 - base : 0), h1 = (u1 - base < a.heads[part] ? u1 - base : a.heads[part]);
-            if (h0 >= h1) continue;
+        for (;;) {
             /* Pair i of the lane is (x[i], x[4 + i]) with SPLIT, (x[2 i], x[2 i + 1]) without. */
             float k00[4], k01[4], k10[4], k11[4];
             if (NORM) {
@@ -195,28 +227,10 @@ k_qk_norm_rope_axes(const __grid_constant__ Rows a, const __grid_constant__ Plan
                     k01[i] = k11[i] = sn[i];
                 }
             }
-            const uint16_t *in = a.in[part] + (size_t)row * a.ldi;
             uint16_t *out = a.out[part] + (size_t)row * a.ldo[part];
-            for (int h = h0; h < h1; h += kInFlight * GROUPS) {
-                uint2 va[kInFlight], vb[kInFlight];
+            for (;;) {
 #pragma unroll
-                for (int i = 0; i < kInFlight; i++) {
-                    const int hh = h + i * GROUPS + grp;
-                    va[i] = vb[i] = make_uint2(0u, 0u);
-                    if (hh < h1) {
-                        const uint16_t *src = in + hh * HD;
-                        if (SPLIT) {
-                            va[i] = *reinterpret_cast<const uint2 *>(src + d0);
-                            vb[i] = *reinterpret_cast<const uint2 *>(src + d1);
-                        } else {
-                            const uint4 v = *reinterpret_cast<const uint4 *>(src + d0);
-                            va[i] = make_uint2(v.x, v.y);
-                            vb[i] = make_uint2(v.z, v.w);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < kInFlight; i++) {
+                for (int i = 0; i < FLIGHT; i++) {
                     const int hh = h + i * GROUPS + grp;
                     float x[8] = {bf_lo(va[i].x), bf_hi(va[i].x), bf_lo(va[i].y), bf_hi(va[i].y),
                                   bf_lo(vb[i].x), bf_hi(vb[i].x), bf_lo(vb[i].y), bf_hi(vb[i].y)};
@@ -248,7 +262,16 @@ k_qk_norm_rope_axes(const __grid_constant__ Rows a, const __grid_constant__ Plan
                         }
                     }
                 }
+                h += FLIGHT * GROUPS;
+                if (h >= h1) break;
+                load();
             }
+            /* The K heads of the chunk, when it began among the Q heads. */
+            if (part || u1 <= a.heads[0] || a.heads[1] == 0) break;
+            part = 1;
+            h = 0;
+            h1 = u1 - a.heads[0] < a.heads[1] ? u1 - a.heads[0] : a.heads[1];
+            load();
         }
     }
 }
@@ -442,7 +465,8 @@ extern "C" int iris_b200_qk_norm_rope_axes(uint16_t *q_out, int ldqo, uint16_t *
         return after_launch(op) ? IRIS_B200_OK : IRIS_B200_ECUDA;
     }
     /* A row is cut into as many warps as it takes to fill the device once. */
-    const long long slots = (long long)g.sm_count * kBlocksPerSM * (kThreads / 32);
+    const int per_sm = split_half ? Shape<true>::kBlocks : Shape<false>::kBlocks;
+    const long long slots = (long long)g.sm_count * per_sm * (kThreads / 32);
     const int groups = 32 / (head_dim / 8);
     int chunks = (int)((slots + seq - 1) / seq);
     const int most = (per_row + groups - 1) / groups;
@@ -451,7 +475,7 @@ extern "C" int iris_b200_qk_norm_rope_axes(uint16_t *q_out, int ldqo, uint16_t *
     a.chunk = (a.chunk + groups - 1) / groups * groups;
     a.chunks = (per_row + a.chunk - 1) / a.chunk;
     long long blocks = ((long long)seq * a.chunks + kThreads / 32 - 1) / (kThreads / 32);
-    if (blocks > (long long)g.sm_count * kBlocksPerSM) blocks = (long long)g.sm_count * kBlocksPerSM;
+    if (blocks > (long long)g.sm_count * per_sm) blocks = (long long)g.sm_count * per_sm;
     Launch l((unsigned)blocks);
     const bool split = split_half != 0, norm = wq != NULL;
     const cudaError_t err = head_dim == 64    ? launch_rows<64>(l.cfg, a, plan, split, norm)
