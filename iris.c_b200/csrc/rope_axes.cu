@@ -48,6 +48,15 @@ struct Plan {
     unsigned char axis[kMaxPairs];
 };
 
+/* An address inside the launch's parameters as a plain one: lanes that read
+ * different entries through the constant cache would be served one after the
+ * other (768 x 60 heads: 11.0 us so, 9.1 us through loads). */
+template <typename T>
+__device__ __forceinline__ const T *plain(const T *param) {
+    asm("" : "+l"(param));
+    return param;
+}
+
 /* cos and sin of the phase p * turn. */
 __device__ __forceinline__ void turn_of(int p, Turn t, float &cs, float &sn) {
     /* Bits 32 to 63 of the phase plus an eighth of a turn: two bits of quadrant, then the angle from -pi / 4 up. */
@@ -83,8 +92,8 @@ k_rope_tables(float *__restrict__ cos_out, float *__restrict__ sin_out, const in
     int axis[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; i++) {
-        turn[i] = plan.turn[j + i];
-        axis[i] = plan.axis[j + i];
+        turn[i] = plain(plan.turn)[j + i];
+        axis[i] = plain(plan.axis)[j + i];
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long stride = (long long)gridDim.x * rows_per_block;
@@ -158,8 +167,8 @@ k_qk_norm_rope_axes(const __grid_constant__ Rows a, const __grid_constant__ Plan
     int axis[PPL];
 #pragma unroll
     for (int i = 0; i < PPL; i++) {
-        turn[i] = plan.turn[lane * PPL + i];
-        axis[i] = plan.axis[lane * PPL + i];
+        turn[i] = plain(plan.turn)[lane * PPL + i];
+        axis[i] = plain(plan.axis)[lane * PPL + i];
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long items = (long long)a.seq * a.chunks;
@@ -303,7 +312,7 @@ k_qk_norm_rope_axes_any(const __grid_constant__ Rows a, const __grid_constant__ 
         for (int j = lane; j < half; j += 32) {
             const int i0 = split_half ? j : 2 * j, i1 = split_half ? j + half : 2 * j + 1;
             float cs, sn;
-            turn_of(a.pos[(size_t)row * plan.n + plan.axis[j]], plan.turn[j], cs, sn);
+            turn_of(a.pos[(size_t)row * plan.n + plain(plan.axis)[j]], plain(plan.turn)[j], cs, sn);
             const float x0 = bf2f(in[i0]) * (w ? inv * w[i0] : 1.0f), x1 = bf2f(in[i1]) * (w ? inv * w[i1] : 1.0f);
             out[i0] = (uint16_t)cvt_bf16x2(x0 * cs - x1 * sn, 0.0f);
             out[i1] = (uint16_t)cvt_bf16x2(x1 * cs + x0 * sn, 0.0f);
@@ -464,15 +473,15 @@ extern "C" int iris_b200_qk_norm_rope_axes(uint16_t *q_out, int ldqo, uint16_t *
         k_qk_norm_rope_axes_any<<<(unsigned)blocks, kThreads, 0, g.stream>>>(a, plan, head_dim, split_half);
         return after_launch(op) ? IRIS_B200_OK : IRIS_B200_ECUDA;
     }
-    /* A row is cut into as many warps as it takes to fill the device once. */
+    /* A row is cut into as many warps as it takes to fill the device once, in
+     * pieces of whole batches (768 x 60 heads: 16 heads per warp 7.8 us, 12 heads
+     * 9.1, 20 heads 8.8). */
     const int per_sm = split_half ? Shape<true>::kBlocks : Shape<false>::kBlocks;
     const long long slots = (long long)g.sm_count * per_sm * (kThreads / 32);
-    const int groups = 32 / (head_dim / 8);
-    int chunks = (int)((slots + seq - 1) / seq);
-    const int most = (per_row + groups - 1) / groups;
-    if (chunks > most) chunks = most;
-    a.chunk = (per_row + chunks - 1) / chunks;
-    a.chunk = (a.chunk + groups - 1) / groups * groups;
+    const int batch = (split_half ? Shape<true>::kInFlight : Shape<false>::kInFlight) * (32 / (head_dim / 8));
+    const long long chunks = (slots + seq - 1) / seq;
+    a.chunk = (int)((per_row + chunks - 1) / chunks);
+    a.chunk = (a.chunk + batch - 1) / batch * batch;
     a.chunks = (per_row + a.chunk - 1) / a.chunk;
     long long blocks = ((long long)seq * a.chunks + kThreads / 32 - 1) / (kThreads / 32);
     if (blocks > (long long)g.sm_count * per_sm) blocks = (long long)g.sm_count * per_sm;
