@@ -163,15 +163,22 @@ __device__ __forceinline__ void score_tile(const Select &p, const double *qf, co
 #pragma unroll
         for (int g = 0; g < HD / 16; g++)
             k[g] = krow ? __ldg(reinterpret_cast<const float4 *>(krow + 16 * g + e0)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        /* (Two sums per tile, so that a product does not wait for the one before.) */
+        double odd[2][2] = {{0.0, 0.0}, {0.0, 0.0}};
 #pragma unroll
         for (int g = 0; g < HD / 16; g++) {
             const float b[4] = {k[g].x, k[g].y, k[g].z, k[g].w};
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const double bv = (double)b[i];
-                mma_f64(d[0], qf[(4 * g + i) * 32 + lane], bv);
-                if (tiles > 1) mma_f64(d[1], qf[(p.steps + 4 * g + i) * 32 + lane], bv);
+                mma_f64(i & 1 ? odd[0] : d[0], qf[(4 * g + i) * 32 + lane], bv);
+                if (tiles > 1) mma_f64(i & 1 ? odd[1] : d[1], qf[(p.steps + 4 * g + i) * 32 + lane], bv);
             }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            d[m][0] += odd[m][0];
+            d[m][1] += odd[m][1];
         }
     } else {
         for (int s = 0; s < p.steps; s++) {
@@ -229,164 +236,193 @@ struct Team {
             b = c[2 * w + 1] > b ? c[2 * w + 1] : b;
         }
     }
-    /* The smallest of lo and the largest of hi over the team: high words, then the low words that go with them. */
-    __device__ __forceinline__ void span(unsigned long long &lo, unsigned long long &hi) {
-        unsigned h = (unsigned)(hi >> 32), l = ~(unsigned)(lo >> 32);
-        most(h, l);
-        unsigned h2 = (unsigned)(hi >> 32) == h ? (unsigned)hi : 0u, l2 = ~(unsigned)(lo >> 32) == l ? ~(unsigned)lo : 0u;
-        most(h2, l2);
-        hi = (unsigned long long)h << 32 | h2;
-        lo = (unsigned long long)~l << 32 | ~l2;
-    }
 };
 
 static constexpr int kBins = 256;
-/* Bin of a score: (float)kBins / range may round up, hence the limit. Monotone: each operation rounds monotonically. */
+/* Bin of a score. Monotone: each operation rounds monotonically; per = kBins / range may round up, hence the limit. */
 __device__ __forceinline__ int bin_of(float f, float low, float per) {
     const int b = (int)((f - low) * per);
     return b < kBins - 1 ? b : kBins - 1;
 }
+/* Scratch of a team in shared memory. */
+struct TeamScratch {
+    unsigned counts[4 * kSelWarps];
+    unsigned hist[kBins];
+    unsigned found;
+    int candidates[32];
+};
 
-/* The score of a key that is neither 0 nor all ones, to fp32: keeps the order. */
-__device__ __forceinline__ float score_of(unsigned long long key) {
-    return (float)__longlong_as_double((long long)((key >> 63) ? key & 0x7FFFFFFFFFFFFFFFull : ~key));
+/* The score of a key from its upper word, to 20 bits, as fp32 (clamped to its
+ * range): never out of order. */
+__device__ __forceinline__ float score_of(uint32_t high) {
+    const uint32_t flip = ~(uint32_t)((int)high >> 31);             /* negative scores are stored inverted */
+    uint32_t t = (high ^ flip) & 0x7FFFFFFFu;                       /* exponent and upper mantissa of the fp64 magnitude */
+    t = t < 0x38000000u ? 0x38000000u : (t > 0x47EFFFFFu ? 0x47EFFFFFu : t);
+    return __uint_as_float((t - 0x38000000u) << 3 | (flip & 0x80000000u));
 }
-__device__ __forceinline__ uint32_t ordered(float f) {
-    const uint32_t b = __float_as_uint(f);
-    return (b >> 31) ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float unordered(uint32_t b) { return __uint_as_float((b >> 31) ? b & 0x7FFFFFFFu : ~b); }
+__device__ __forceinline__ uint32_t high_of(const unsigned long long *key) { return reinterpret_cast<const uint32_t *>(key)[1]; }
 
 /* The list of one row: its keys (0: not eligible, all ones: always taken) are
  * in shared memory, a run of them for every warp of the team. A histogram of
  * the scores over 256 equal bins between the lowest and the highest narrows the
- * place of the topk-th down to one bin; where only a part of the bin is
- * wanted, a search over the bits of its keys finds the cut. */
-__device__ __forceinline__ void choose(const Select &p, Team t, const unsigned long long *keys, unsigned *hist, int *list) {
+ * place of the topk-th down to one bin, on the upper words of the keys alone.
+ * Where only a part of that bin is wanted its keys are ranked in full: up to 32
+ * by one warp, more by a search over their bits. The chosen keys of the bin are
+ * turned into all ones, and everything above the bin is taken. */
+__device__ __forceinline__ void choose(const Select &p, Team t, unsigned long long *keys, TeamScratch &sc, int *list) {
     const int lane = threadIdx.x & 31;
     const int run = ((p.k_blocks + t.warps - 1) / t.warps + 31) & ~31;
     const int j0 = t.me * run < p.k_blocks ? t.me * run : p.k_blocks;
     const int j1 = j0 + run < p.k_blocks ? j0 + run : p.k_blocks;
+    const unsigned before = (1u << lane) - 1u;
     unsigned eligible = 0, kept = 0, x, y, top = 0, bottom = 0;
     for (int j = j0 + lane; j < j1; j += 32) {
-        const unsigned long long k = keys[j];
-        eligible += k != 0ull;
-        kept += k == ~0ull;
-        if (k != 0ull && k != ~0ull) {
-            const uint32_t f = ordered(score_of(k));
-            top = f > top ? f : top;
-            bottom = ~f > bottom ? ~f : bottom;
+        const uint32_t h = high_of(keys + j);
+        eligible += h != 0u;
+        kept += h == ~0u;
+        if (h != 0u && h != ~0u) {
+            top = h > top ? h : top;
+            bottom = ~h > bottom ? ~h : bottom;
         }
     }
-    for (int i = t.me * 32 + lane; i < kBins; i += t.warps * 32) hist[i] = 0u;
+    for (int i = t.me * 32 + lane; i < kBins; i += t.warps * 32) sc.hist[i] = 0u;
+    if (t.me == 0 && lane == 0) sc.found = 0u;
     __syncwarp();
     t.sum(eligible, kept, x, y);
-    t.most(top, bottom);
     const unsigned want = (unsigned)p.topk < eligible ? (unsigned)p.topk : eligible;
-    unsigned long long cut = 1ull;               /* keys above the cut are taken, equal ones from the lowest index */
+    uint32_t bar = 0u;                           /* upper words above it are taken */
     if (want < eligible) {
-        unsigned long long lo = 1ull, hi = ~0ull;          /* lo is reached by enough keys; the answer is not above hi */
-        const float low = unordered(~bottom), range = unordered(top) - low;
-        if (want <= kept) {
-            lo = ~0ull;                                    /* the places are taken already */
-        } else if (range > 0.0f && range < 1e30f) {
-            const float per = (float)kBins / range;
-            for (int j = j0 + lane; j < j1; j += 32) {
-                const unsigned long long k = keys[j];
-                if (k != 0ull && k != ~0ull) atomicAdd(hist + bin_of(score_of(k), low, per), 1u);
+        bar = ~1u;
+        if (want > kept) {
+            t.most(top, bottom);
+            const unsigned left = want - kept;           /* places for scores */
+            const float low = score_of(~bottom), range = score_of(top) - low;
+            const float per = range > 0.0f && range < 1e30f ? (float)kBins / range : 0.0f;
+            int bin = 0;
+            unsigned in_bin = eligible - kept, take = left;
+            if (per > 0.0f) {
+                for (int j = j0 + lane; j < j1; j += 32) {
+                    const uint32_t h = high_of(keys + j);
+                    if (h != 0u && h != ~0u) atomicAdd(sc.hist + bin_of(score_of(h), low, per), 1u);
+                }
+                __syncwarp();
+                t.sync();
+                /* Scores in the bins above mine, eight bins a lane from the top. */
+                unsigned n[8], mine = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    n[i] = sc.hist[kBins - 1 - (lane * 8 + i)];
+                    mine += n[i];
+                }
+                unsigned above = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned v = __shfl_up_sync(0xffffffffu, above, o);
+                    if (lane >= o) above += v;
+                }
+                above -= mine;
+                bin = -1;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (above < left && above + n[i] >= left) {      /* one lane holds the bin of the last place */
+                        bin = kBins - 1 - (lane * 8 + i);
+                        in_bin = n[i];
+                        take = left - above;
+                    }
+                    above += n[i];
+                }
+                const int src = __ffs(__ballot_sync(0xffffffffu, bin >= 0)) - 1;
+                bin = __shfl_sync(0xffffffffu, bin, src);
+                in_bin = __shfl_sync(0xffffffffu, in_bin, src);
+                take = __shfl_sync(0xffffffffu, take, src);
             }
-            t.sync();
+            /* The upper words of the bin, and where its keys are when they have to be ranked. */
+            const bool rank = take < in_bin && in_bin <= 32u;
+            unsigned most = 0, least = 0;
+            for (int j = j0 + lane; j < j1; j += 32) {
+                const uint32_t h = high_of(keys + j);
+                if (h == 0u || h == ~0u || (per > 0.0f && bin_of(score_of(h), low, per) != bin)) continue;
+                most = h > most ? h : most;
+                least = ~h > least ? ~h : least;
+                if (rank) sc.candidates[atomicAdd(&sc.found, 1u)] = j;
+            }
             __syncwarp();
-            /* Scores in the bins above mine, eight bins a lane from the top. */
-            unsigned n[8], mine = 0;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                n[i] = hist[kBins - 1 - (lane * 8 + i)];
-                mine += n[i];
-            }
-            unsigned above = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned v = __shfl_up_sync(0xffffffffu, above, o);
-                if (lane >= o) above += v;
-            }
-            above -= mine;
-            const unsigned left = want - kept;             /* places for scores; one lane holds the bin of the last */
-            int bin = -1;
-            unsigned in_bin = 0, take = 0;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if (above < left && above + n[i] >= left) {
-                    bin = kBins - 1 - (lane * 8 + i);
-                    in_bin = n[i];
-                    take = left - above;
+            t.most(most, least);
+            bar = take < in_bin ? most : ~least - 1u;
+            if (rank) {
+                if (t.me == 0) {
+                    const int j = lane < (int)in_bin ? sc.candidates[lane] : -1;
+                    const unsigned long long k = j >= 0 ? keys[j] : 0ull;
+                    unsigned ahead = 0;
+                    for (int c = 0; c < (int)in_bin; c++) {
+                        const unsigned long long k2 = __shfl_sync(0xffffffffu, k, c);
+                        const int j2 = __shfl_sync(0xffffffffu, j, c);
+                        ahead += k2 > k || (k2 == k && j2 < j);
+                    }
+                    __syncwarp();
+                    if (j >= 0 && ahead < take) keys[j] = ~0ull;
+                    __syncwarp();
                 }
-                above += n[i];
-            }
-            const int src = __ffs(__ballot_sync(0xffffffffu, bin >= 0)) - 1;
-            bin = __shfl_sync(0xffffffffu, bin, src);
-            in_bin = __shfl_sync(0xffffffffu, in_bin, src);
-            take = __shfl_sync(0xffffffffu, take, src);
-            /* The keys of that bin span [lo, hi]. */
-            unsigned long long a = 0ull, b = ~0ull;
-            for (int j = j0 + lane; j < j1; j += 32) {
-                const unsigned long long k = keys[j];
-                if (k != 0ull && k != ~0ull && bin_of(score_of(k), low, per) == bin) {
-                    a = k > a ? k : a;
-                    b = k < b ? k : b;
+                t.sync();
+            } else if (take < in_bin) {
+                /* Keys of the bin: the largest value that `take` of them reach, three thresholds a step (two bits). */
+                unsigned long long lo = (unsigned long long)~least << 32, hi = (unsigned long long)most << 32 | 0xFFFFFFFFull;
+                while (lo < hi) {
+                    const unsigned long long q = (hi - lo) / 4 + 1;     /* lo < t1 <= t2 <= t3 <= hi */
+                    const unsigned long long t1 = lo + q, t2 = hi - t1 < q ? hi : t1 + q, t3 = hi - t2 < q ? hi : t2 + q;
+                    unsigned n12 = 0, n3 = 0;
+                    for (int j = j0 + lane; j < j1; j += 32) {
+                        const unsigned long long k = keys[j];
+                        if ((uint32_t)(k >> 32) > most) continue;
+                        n12 += (unsigned)(k >= t1) + ((unsigned)(k >= t2) << 16);
+                        n3 += k >= t3;
+                    }
+                    t.sum(n12, n3, x, y);
+                    const unsigned n1 = n12 & 0xffffu, n2 = n12 >> 16;
+                    if (n3 >= take) {
+                        lo = t3;
+                    } else if (n2 >= take) {
+                        lo = t2;
+                        hi = t3 - 1ull;
+                    } else if (n1 >= take) {
+                        lo = t1;
+                        hi = t2 - 1ull;
+                    } else {
+                        hi = t1 - 1ull;
+                    }
                 }
-            }
-            t.span(b, a);
-            lo = b;
-            hi = take == in_bin ? b : a;
-        }
-        while (lo < hi) {                                  /* three thresholds a step: two bits */
-            const unsigned long long q = (hi - lo) / 4 + 1;     /* lo < t1 <= t2 <= t3 <= hi */
-            const unsigned long long t1 = lo + q, t2 = hi - t1 < q ? hi : t1 + q, t3 = hi - t2 < q ? hi : t2 + q;
-            unsigned n12 = 0, n3 = 0;
-            for (int j = j0 + lane; j < j1; j += 32) {
-                const unsigned long long k = keys[j];
-                n12 += (unsigned)(k >= t1) + ((unsigned)(k >= t2) << 16);
-                n3 += k >= t3;
-            }
-            t.sum(n12, n3, x, y);
-            const unsigned n1 = n12 & 0xffffu, n2 = n12 >> 16;
-            if (n3 >= want) {
-                lo = t3;
-                if (n3 == want) break;
-            } else if (n2 >= want) {
-                lo = t2;
-                hi = t3 - 1ull;
-                if (n2 == want) break;
-            } else if (n1 >= want) {
-                lo = t1;
-                hi = t2 - 1ull;
-                if (n1 == want) break;
-            } else {
-                hi = t1 - 1ull;
+                /* Above the cut all, equal to it from the lowest index. */
+                unsigned over = 0, equal = 0, over_before, equal_before;
+                for (int j = j0 + lane; j < j1; j += 32) {
+                    const unsigned long long k = keys[j];
+                    over += k > lo && (uint32_t)(k >> 32) <= most;
+                    equal += k == lo;
+                }
+                t.sum(over, equal, over_before, equal_before);
+                unsigned equal_left = take - over;
+                equal_left = equal_before < equal_left ? equal_left - equal_before : 0u;
+                for (int j = j0; j < j1; j += 32) {
+                    const unsigned long long k = j + lane < j1 ? keys[j + lane] : 0ull;
+                    const unsigned eq = __ballot_sync(0xffffffffu, k == lo);
+                    if ((k > lo && (uint32_t)(k >> 32) <= most) || (k == lo && __popc(eq & before) < equal_left)) keys[j + lane] = ~0ull;
+                    equal_left -= __popc(eq) < equal_left ? __popc(eq) : equal_left;
+                }
+                __syncwarp();
             }
         }
-        cut = lo;
     }
-    unsigned above = 0, equal = 0, above_before, equal_before;
-    for (int j = j0 + lane; j < j1; j += 32) {
-        const unsigned long long k = keys[j];
-        above += k > cut;
-        equal += k == cut;
+    /* Each warp writes the blocks of its run behind those of the warps before it. */
+    unsigned done = 0, none = 0;
+    if (t.warps > 1) {
+        unsigned taken = 0;
+        for (int j = j0 + lane; j < j1; j += 32) taken += high_of(keys + j) > bar;
+        t.sum(taken, none, done, y);
     }
-    t.sum(above, equal, above_before, equal_before);
-    const unsigned equal_taken = want - above;   /* of the keys equal to the cut */
-    unsigned done = above_before + (equal_before < equal_taken ? equal_before : equal_taken);
-    unsigned equal_left = equal_before < equal_taken ? equal_taken - equal_before : 0u;
-    const unsigned before = (1u << lane) - 1u;
     for (int j = j0; j < j1; j += 32) {
-        const unsigned long long k = j + lane < j1 ? keys[j + lane] : 0ull;
-        const unsigned eq = __ballot_sync(0xffffffffu, k == cut);
-        const bool take = k > cut || (k == cut && __popc(eq & before) < equal_left);
+        const bool take = j + lane < j1 && high_of(keys + j + lane) > bar;
         const unsigned m = __ballot_sync(0xffffffffu, take);
         if (take) list[done + __popc(m & before)] = j + lane;
         done += __popc(m);
-        equal_left -= __popc(eq) < equal_left ? __popc(eq) : equal_left;
     }
     for (unsigned i = want + t.me * 32 + lane; i < (unsigned)p.topk; i += t.warps * 32) list[i] = -1;
 }
@@ -396,8 +432,7 @@ __global__ void __launch_bounds__(kSelThreads, 2)
 k_block_select(const __grid_constant__ Select p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    __shared__ unsigned team_counts[kSelWarps][4 * kSelWarps];
-    __shared__ unsigned team_hist[kSelWarps][kBins];
+    __shared__ TeamScratch scratch[kSelWarps];
     /* The rows as operand fragments [tile][product][lane], then [own_rows][k_blocks] keys. */
     double *qf = reinterpret_cast<double *>(smem_raw);
     const int tiles = p.rows > 8 ? 2 : 1;
@@ -459,11 +494,12 @@ k_block_select(const __grid_constant__ Select p) {
     __syncwarp();
     if (p.ctas > 1) sm100::cluster_sync_all();
     else __syncthreads();
-    Team t = {warp % p.team, p.team, 1 + warp / p.team, team_counts[warp / p.team], 0u};
+    TeamScratch &sc = scratch[warp / p.team];
+    Team t = {warp % p.team, p.team, 1 + warp / p.team, sc.counts, 0u};
     for (int r = warp / p.team; r < p.own_rows; r += kSelWarps / p.team) {
         const int row = r * p.ctas + rank;
         if (row < p.rows && row_of(p, g, r0 + row, &qb, &head))
-            choose(p, t, keys + (size_t)r * p.k_blocks, team_hist[warp / p.team], p.list + ((size_t)head * p.q_blocks + qb) * p.topk);
+            choose(p, t, keys + (size_t)r * p.k_blocks, sc, p.list + ((size_t)head * p.q_blocks + qb) * p.topk);
         __syncwarp();
         t.sync();
     }
