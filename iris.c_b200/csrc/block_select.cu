@@ -246,11 +246,12 @@ __device__ __forceinline__ int bin_of(float f, float low, float per) {
 }
 /* Scratch of a team in shared memory. */
 struct TeamScratch {
+    alignas(16) unsigned hist[kBins];
     unsigned counts[4 * kSelWarps];
-    unsigned hist[kBins];
     unsigned found;
     int candidates[32];
 };
+static constexpr uint32_t kOut = 0u, kTaken = ~0u;       /* upper words of keys that are no scores */
 
 /* The score of a key from its upper word, to 20 bits, as fp32 (clamped to its
  * range): never out of order. */
@@ -268,88 +269,107 @@ __device__ __forceinline__ uint32_t high_of(const unsigned long long *key) { ret
  * place of the topk-th down to one bin, on the upper words of the keys alone.
  * Where only a part of that bin is wanted its keys are ranked in full: up to 32
  * by one warp, more by a search over their bits. The chosen keys of the bin are
- * turned into all ones, and everything above the bin is taken. */
+ * turned into all ones, and everything above the bin is taken.
+ * WORDS > 0: a lane holds that many upper words in registers, which covers the
+ * run, and every pass over them is straight-line code (with the words read from
+ * shared memory in loops, a row of 264 blocks took 5 us instead of 3.3). */
+template <int WORDS>
 __device__ __forceinline__ void choose(const Select &p, Team t, unsigned long long *keys, TeamScratch &sc, int *list) {
     const int lane = threadIdx.x & 31;
     const int run = ((p.k_blocks + t.warps - 1) / t.warps + 31) & ~31;
     const int j0 = t.me * run < p.k_blocks ? t.me * run : p.k_blocks;
     const int j1 = j0 + run < p.k_blocks ? j0 + run : p.k_blocks;
     const unsigned before = (1u << lane) - 1u;
-    unsigned eligible = 0, kept = 0, x, y, top = 0, bottom = 0;
-    for (int j = j0 + lane; j < j1; j += 32) {
-        const uint32_t h = high_of(keys + j);
-        eligible += h != 0u;
-        kept += h == ~0u;
-        if (h != 0u && h != ~0u) {
-            top = h > top ? h : top;
-            bottom = ~h > bottom ? ~h : bottom;
-        }
+    uint32_t words[WORDS > 0 ? WORDS : 1];
+    if (WORDS > 0) {
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) words[i] = j0 + 32 * i + lane < j1 ? high_of(keys + j0 + 32 * i + lane) : kOut;
     }
-    for (int i = t.me * 32 + lane; i < kBins; i += t.warps * 32) sc.hist[i] = 0u;
+    /* fn(i, block, word) for this lane's blocks, kOut behind the last. */
+    auto each = [&](auto fn) {
+        if (WORDS > 0) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) fn(i, j0 + 32 * i + lane, words[i]);
+        } else {
+            for (int j = j0 + lane; j < j1; j += 32) fn(0, j, high_of(keys + j));
+        }
+    };
+    unsigned eligible = 0, kept = 0, x, y, top = 0, bottom = 0;
+    each([&](int, int, uint32_t w) {
+        eligible += w != kOut;
+        kept += w == kTaken;
+        const bool score = w != kOut && w != kTaken;
+        top = score && w > top ? w : top;
+        bottom = score && ~w > bottom ? ~w : bottom;
+    });
+    for (int i = t.me * 32 + lane; i < kBins / 4; i += t.warps * 32) reinterpret_cast<uint4 *>(sc.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
     if (t.me == 0 && lane == 0) sc.found = 0u;
     __syncwarp();
     t.sum(eligible, kept, x, y);
     const unsigned want = (unsigned)p.topk < eligible ? (unsigned)p.topk : eligible;
-    uint32_t bar = 0u;                           /* upper words above it are taken */
+    uint32_t bar = kOut;                         /* upper words above it are taken */
     if (want < eligible) {
-        bar = ~1u;
+        bar = kTaken - 1u;
         if (want > kept) {
             t.most(top, bottom);
             const unsigned left = want - kept;           /* places for scores */
             const float low = score_of(~bottom), range = score_of(top) - low;
+            /* (Without a span, or an infinite one, everything is in bin 0.) */
             const float per = range > 0.0f && range < 1e30f ? (float)kBins / range : 0.0f;
-            int bin = 0;
-            unsigned in_bin = eligible - kept, take = left;
-            if (per > 0.0f) {
-                for (int j = j0 + lane; j < j1; j += 32) {
-                    const uint32_t h = high_of(keys + j);
-                    if (h != 0u && h != ~0u) atomicAdd(sc.hist + bin_of(score_of(h), low, per), 1u);
-                }
-                __syncwarp();
-                t.sync();
-                /* Scores in the bins above mine, eight bins a lane from the top. */
-                unsigned n[8], mine = 0;
+            int bins[WORDS > 0 ? WORDS : 1];             /* -1: no score */
+            auto bin_at = [&](uint32_t w) { return w == kOut || w == kTaken ? -1 : per > 0.0f ? bin_of(score_of(w), low, per) : 0; };
+            each([&](int i, int, uint32_t w) {
+                const int b = bin_at(w);
+                if (WORDS > 0) bins[i] = b;
+                if (b >= 0) atomicAdd(sc.hist + b, 1u);
+            });
+            __syncwarp();
+            t.sync();
+            /* Scores in the bins above mine, eight bins a lane from the top; one lane holds the bin of the last place. */
+            unsigned n[8], mine = 0;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    n[i] = sc.hist[kBins - 1 - (lane * 8 + i)];
-                    mine += n[i];
-                }
-                unsigned above = mine;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned v = __shfl_up_sync(0xffffffffu, above, o);
-                    if (lane >= o) above += v;
-                }
-                above -= mine;
-                bin = -1;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (above < left && above + n[i] >= left) {      /* one lane holds the bin of the last place */
-                        bin = kBins - 1 - (lane * 8 + i);
-                        in_bin = n[i];
-                        take = left - above;
-                    }
-                    above += n[i];
-                }
-                const int src = __ffs(__ballot_sync(0xffffffffu, bin >= 0)) - 1;
-                bin = __shfl_sync(0xffffffffu, bin, src);
-                in_bin = __shfl_sync(0xffffffffu, in_bin, src);
-                take = __shfl_sync(0xffffffffu, take, src);
+            for (int i = 0; i < 2; i++) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(sc.hist + kBins - 8 * lane - 4 * (i + 1));
+                n[4 * i] = v.w;
+                n[4 * i + 1] = v.z;
+                n[4 * i + 2] = v.y;
+                n[4 * i + 3] = v.x;
+                mine += v.x + v.y + v.z + v.w;
             }
+            unsigned above = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned v = __shfl_up_sync(0xffffffffu, above, o);
+                if (lane >= o) above += v;
+            }
+            above -= mine;
+            unsigned found = 0;                          /* bin + 1 in bits 0 to 8, places left in it above */
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (above < left && above + n[i] >= left) found = (unsigned)(kBins - (lane * 8 + i)) | (left - above) << 9 | (n[i] == left - above ? 1u << 31 : 0u);
+                above += n[i];
+            }
+            found = __reduce_max_sync(0xffffffffu, found);
+            const int bin = (int)(found & 511u) - 1;
+            const unsigned take = (found >> 9) & 0x3FFFFFu;
+            const bool whole = found >> 31;
             /* The upper words of the bin, and where its keys are when they have to be ranked. */
-            const bool rank = take < in_bin && in_bin <= 32u;
             unsigned most = 0, least = 0;
-            for (int j = j0 + lane; j < j1; j += 32) {
-                const uint32_t h = high_of(keys + j);
-                if (h == 0u || h == ~0u || (per > 0.0f && bin_of(score_of(h), low, per) != bin)) continue;
-                most = h > most ? h : most;
-                least = ~h > least ? ~h : least;
-                if (rank) sc.candidates[atomicAdd(&sc.found, 1u)] = j;
-            }
+            each([&](int i, int j, uint32_t w) {
+                const bool in = (WORDS > 0 ? bins[i] : bin_at(w)) == bin;
+                most = in && w > most ? w : most;
+                least = in && ~w > least ? ~w : least;
+                if (in && !whole) {
+                    const unsigned at = atomicAdd(&sc.found, 1u);
+                    if (at < 32u) sc.candidates[at] = j;
+                }
+            });
             __syncwarp();
             t.most(most, least);
-            bar = take < in_bin ? most : ~least - 1u;
-            if (rank) {
+            bar = whole ? ~least - 1u : most;
+            t.sync();
+            const unsigned in_bin = whole ? 0u : sc.found;
+            if (!whole && in_bin <= 32u) {
                 if (t.me == 0) {
                     const int j = lane < (int)in_bin ? sc.candidates[lane] : -1;
                     const unsigned long long k = j >= 0 ? keys[j] : 0ull;
@@ -364,7 +384,7 @@ __device__ __forceinline__ void choose(const Select &p, Team t, unsigned long lo
                     __syncwarp();
                 }
                 t.sync();
-            } else if (take < in_bin) {
+            } else if (!whole) {
                 /* Keys of the bin: the largest value that `take` of them reach, three thresholds a step (two bits). */
                 unsigned long long lo = (unsigned long long)~least << 32, hi = (unsigned long long)most << 32 | 0xFFFFFFFFull;
                 while (lo < hi) {
@@ -409,20 +429,36 @@ __device__ __forceinline__ void choose(const Select &p, Team t, unsigned long lo
                 }
                 __syncwarp();
             }
+            /* The words of ranked keys have changed. */
+            if (WORDS > 0 && !whole) {
+#pragma unroll
+                for (int i = 0; i < WORDS; i++) words[i] = j0 + 32 * i + lane < j1 ? high_of(keys + j0 + 32 * i + lane) : kOut;
+            }
         }
     }
     /* Each warp writes the blocks of its run behind those of the warps before it. */
     unsigned done = 0, none = 0;
     if (t.warps > 1) {
         unsigned taken = 0;
-        for (int j = j0 + lane; j < j1; j += 32) taken += high_of(keys + j) > bar;
+        each([&](int, int, uint32_t w) { taken += w > bar; });
         t.sum(taken, none, done, y);
     }
-    for (int j = j0; j < j1; j += 32) {
-        const bool take = j + lane < j1 && high_of(keys + j + lane) > bar;
-        const unsigned m = __ballot_sync(0xffffffffu, take);
-        if (take) list[done + __popc(m & before)] = j + lane;
-        done += __popc(m);
+    if (WORDS > 0) {
+        unsigned m[WORDS > 0 ? WORDS : 1];
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) m[i] = __ballot_sync(0xffffffffu, words[i] > bar);
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) {
+            if (words[i] > bar) list[done + __popc(m[i] & before)] = j0 + 32 * i + lane;
+            done += __popc(m[i]);
+        }
+    } else {
+        for (int j = j0; j < j1; j += 32) {
+            const bool take = j + lane < j1 && high_of(keys + j + lane) > bar;
+            const unsigned m = __ballot_sync(0xffffffffu, take);
+            if (take) list[done + __popc(m & before)] = j + lane;
+            done += __popc(m);
+        }
     }
     for (unsigned i = want + t.me * 32 + lane; i < (unsigned)p.topk; i += t.warps * 32) list[i] = -1;
 }
@@ -498,8 +534,19 @@ k_block_select(const __grid_constant__ Select p) {
     Team t = {warp % p.team, p.team, 1 + warp / p.team, sc.counts, 0u};
     for (int r = warp / p.team; r < p.own_rows; r += kSelWarps / p.team) {
         const int row = r * p.ctas + rank;
-        if (row < p.rows && row_of(p, g, r0 + row, &qb, &head))
-            choose(p, t, keys + (size_t)r * p.k_blocks, sc, p.list + ((size_t)head * p.q_blocks + qb) * p.topk);
+        if (row < p.rows && row_of(p, g, r0 + row, &qb, &head)) {
+            unsigned long long *mine = keys + (size_t)r * p.k_blocks;
+            int *list = p.list + ((size_t)head * p.q_blocks + qb) * p.topk;
+            const int words = ((p.k_blocks + p.team - 1) / p.team + 31) / 32;        /* of a lane */
+            if (words <= 4)
+                choose<4>(p, t, mine, sc, list);
+            else if (words <= 9)
+                choose<9>(p, t, mine, sc, list);
+            else if (words <= 16)
+                choose<16>(p, t, mine, sc, list);
+            else
+                choose<0>(p, t, mine, sc, list);
+        }
         __syncwarp();
         t.sync();
     }
