@@ -150,40 +150,59 @@ __device__ __forceinline__ void mma_f64(double d[2], double a, double b) {
                  : "+d"(d[0]), "+d"(d[1]) : "d"(a), "d"(b));
 }
 
-/* Scores of the cluster's rows against the blocks j0 .. j0 + 7 by one warp:
- * d[m] holds row 8 m + lane / 4 and the blocks j0 + 2 (lane & 3), + 1. Product
- * s of a 16-dimension group takes the dimensions 16 g + 4 (lane & 3) + s. qf:
- * the rows as fp64 operand fragments in shared memory. HD 0: any head_dim. */
+/* What a lane needs of a block for a score tile: four dimensions of every
+ * sixteen. HD 0: any head_dim, read where it is used. */
 template <int HD>
-__device__ __forceinline__ void score_tile(const Select &p, const double *qf, const float *krow, int lane, int tiles, double d[2][2]) {
-    d[0][0] = d[0][1] = d[1][0] = d[1][1] = 0.0;
-    const int e0 = (lane & 3) * 4;
-    if (HD > 0) {
-        float4 k[HD / 16 + 1];
+struct Block {
+    float4 v[HD / 16 + 1];
+    const float *row;
+    __device__ __forceinline__ void load(const float *krow, int lane) {
+        row = krow;
 #pragma unroll
         for (int g = 0; g < HD / 16; g++)
-            k[g] = krow ? __ldg(reinterpret_cast<const float4 *>(krow + 16 * g + e0)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        /* (Two sums per tile, so that a product does not wait for the one before.) */
-        double odd[2][2] = {{0.0, 0.0}, {0.0, 0.0}};
+            v[g] = krow ? __ldg(reinterpret_cast<const float4 *>(krow + 16 * g + (lane & 3) * 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+};
+
+/* Scores of the cluster's rows against eight blocks by one warp: d[m] holds row
+ * 8 m + lane / 4 and the blocks 2 (lane & 3), + 1. Product s of a 16-dimension
+ * group takes the dimensions 16 g + 4 (lane & 3) + s. qf: the rows as fp64 operand
+ * fragments in shared memory. */
+template <int HD>
+__device__ __forceinline__ void score_tile(const Select &p, const double *qf, const Block<HD> &k, int lane, int tiles, double d[2][2]) {
+    d[0][0] = d[0][1] = d[1][0] = d[1][1] = 0.0;
+    if (HD > 0) {
+        /* (Several sums per tile, so that a product does not wait for the one before.) */
+        double more[3][2] = {{0.0, 0.0}, {0.0, 0.0}, {0.0, 0.0}};
+        if (tiles > 1) {
 #pragma unroll
-        for (int g = 0; g < HD / 16; g++) {
-            const float b[4] = {k[g].x, k[g].y, k[g].z, k[g].w};
+            for (int g = 0; g < HD / 16; g++) {
+                const float b[4] = {k.v[g].x, k.v[g].y, k.v[g].z, k.v[g].w};
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const double bv = (double)b[i];
-                mma_f64(i & 1 ? odd[0] : d[0], qf[(4 * g + i) * 32 + lane], bv);
-                if (tiles > 1) mma_f64(i & 1 ? odd[1] : d[1], qf[(p.steps + 4 * g + i) * 32 + lane], bv);
+                for (int i = 0; i < 4; i++) {
+                    const double bv = (double)b[i];
+                    mma_f64(i & 1 ? more[0] : d[0], qf[(4 * g + i) * 32 + lane], bv);
+                    mma_f64(i & 1 ? more[1] : d[1], qf[(p.steps + 4 * g + i) * 32 + lane], bv);
+                }
             }
-        }
+            d[1][0] += more[1][0];
+            d[1][1] += more[1][1];
+        } else {
 #pragma unroll
-        for (int m = 0; m < 2; m++) {
-            d[m][0] += odd[m][0];
-            d[m][1] += odd[m][1];
+            for (int g = 0; g < HD / 16; g++) {
+                const float b[4] = {k.v[g].x, k.v[g].y, k.v[g].z, k.v[g].w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) mma_f64(i ? more[i - 1] : d[0], qf[(4 * g + i) * 32 + lane], (double)b[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) d[0][i] += more[1][i] + more[2][i];
         }
+        d[0][0] += more[0][0];
+        d[0][1] += more[0][1];
     } else {
         for (int s = 0; s < p.steps; s++) {
-            const int e = (s >> 2) * 16 + e0 + (s & 3);
-            const double bv = krow && e < p.head_dim ? (double)krow[e] : 0.0;
+            const int e = (s >> 2) * 16 + (lane & 3) * 4 + (s & 3);
+            const double bv = k.row && e < p.head_dim ? (double)k.row[e] : 0.0;
             mma_f64(d[0], qf[s * 32 + lane], bv);
             if (tiles > 1) mma_f64(d[1], qf[(p.steps + s) * 32 + lane], bv);
         }
@@ -478,6 +497,13 @@ k_block_select(const __grid_constant__ Select p) {
     const int g = blockIdx.y;
     const long long r0 = (long long)(blockIdx.x / (unsigned)p.ctas) * p.rows;
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int b0 = rank * p.slice, b1 = b0 + p.slice < p.k_blocks ? b0 + p.slice : p.k_blocks;
+    auto block_at = [&](int j0) -> const float * {
+        const int j = j0 + (lane >> 2);
+        return j < b1 ? p.km + ((size_t)j * p.kv_heads + g) * p.head_dim : nullptr;
+    };
+    Block<HD> next;
+    next.load(block_at(b0 + warp * 8), lane);
     int qb = 0, head = 0;
     /* Four consecutive dimensions of a row at a time: products 4 g .. 4 g + 3 of lane 4 (row mod 8) + quarter. */
     const int quads = p.steps;                       /* per row */
@@ -502,11 +528,11 @@ k_block_select(const __grid_constant__ Select p) {
     }
     if (p.ctas > 1) sm100::cluster_sync_all();           /* every CTA has started: its shared memory may be written */
     else __syncthreads();
-    const int b0 = rank * p.slice, b1 = b0 + p.slice < p.k_blocks ? b0 + p.slice : p.k_blocks;
     for (int j0 = b0 + warp * 8; j0 < b1; j0 += kSelWarps * 8) {
-        const int jb = j0 + (lane >> 2);
+        const Block<HD> k = next;
+        next.load(block_at(j0 + kSelWarps * 8), lane);       /* under the products of this tile */
         double d[2][2];
-        score_tile<HD>(p, qf, jb < b1 ? p.km + ((size_t)jb * p.kv_heads + g) * p.head_dim : nullptr, lane, tiles, d);
+        score_tile<HD>(p, qf, k, lane, tiles, d);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int j = j0 + (lane & 3) * 2 + i;
