@@ -446,10 +446,12 @@ int iris_b200_block_select(int *list, const float *q_means, const float *k_means
  * k_block)) are skipped, in any place; a block listed twice counts twice.
  * key_mask [seq_k] (NULL: all): 0 = ignored key, whatever its K and V rows
  * hold. A query without any key gets a zero row. Every tensor has its own row
- * stride; query head h uses key head h / (heads / kv_heads). q_block 1 gives every query its own list. Not causal. kernel: one
- * of IRIS_B200_KERNEL_*; the tcgen05 kernel serves head_dim 128, k_block 16,
- * 32, 64 or a multiple of 128, strides in multiples of 8 and 16-byte aligned
- * pointers, the general one everything up to head_dim 512. */
+ * stride; out must not overlap the others; query head h uses key head h /
+ * (heads / kv_heads). q_block 1 gives every query its own list. Not causal.
+ * list_len <= 2^30, heads <= 65535. kernel: one of IRIS_B200_KERNEL_*; the
+ * tcgen05 kernel serves head_dim 128, k_block 16, 32, 64 or a multiple of 128,
+ * strides in multiples of 8 and 16-byte aligned pointers, the general one
+ * everything up to head_dim 512. */
 int iris_b200_attention_blocks(uint16_t *out, int ldo, const uint16_t *q, int ldq,
                                const uint16_t *k, int ldk, const uint16_t *v, int ldv,
                                int seq_q, int seq_k, int heads, int kv_heads, int head_dim, float scale,

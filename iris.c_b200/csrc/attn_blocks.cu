@@ -156,6 +156,7 @@ extern "C" int iris_b200_attention_blocks(uint16_t *out, int ldo, const uint16_t
     if (!(scale > 0.0f) || scale > 3.0e38f) return bad("scale must be positive and finite");
     if (kernel < IRIS_B200_KERNEL_AUTO || kernel > IRIS_B200_KERNEL_GENERIC) return bad("unknown kernel");
     if (heads > 65535) return bad("too many heads");
+    if (list_len > 1 << 30) return bad("list_len above 2^30");
     if (seq_q > 0 && (!out || !q || (seq_k > 0 && (!k || !v)) || (list_len > 0 && !list))) return bad("bad argument");
     BlockAttnArgs a = {};
     a.out = out;

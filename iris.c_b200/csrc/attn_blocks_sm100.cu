@@ -18,10 +18,11 @@
  *   A key tile is 128 rows made of 128 / k_block listed blocks (or a piece of
  *   a longer block), each its own TMA box, so blocks may lie anywhere. The
  *   producer warp reads the list 32 entries at a time, skips what names no
- *   block or holds no valid key, and publishes with every tile one bit per key: zero for rows behind
- *   seq_k, masked rows and the rows of a last tile that no block filled. Their
- *   scores become -inf whatever K holds; their V rows are cleared in shared
- *   memory before the MMA, since a zero probability does not cancel a NaN.
+ *   block or holds no valid key, and publishes with every tile one bit per
+ *   key: zero for rows behind seq_k, masked rows and the rows of a last tile
+ *   that no block filled. Their scores become -inf whatever K holds; their V
+ *   rows are cleared in shared memory before the MMA, since a zero probability
+ *   does not cancel a NaN.
  *
  * Warps (256 threads)
  *   0-3  softmax: thread r owns row r of S / P / O
@@ -156,7 +157,7 @@ __device__ __forceinline__ void producer(const Ctx &c, const Params &p, const Ti
     int j = 0;                          /* tiles published */
     int loads_k = 0, loads_v = 0;       /* tiles whose K / V copies were started */
     /* Q and the first entries of the list are on their way before anything else. */
-    int entry = t.e0 + lane < t.e1 ? __ldg(t.list + t.e0 + lane) : -1;
+    int entry = t.e0 + lane < t.e1 ? t.list[t.e0 + lane] : -1;
     if (lane == 0 && t.e0 < t.e1) {
         mbar_expect_tx(c.bars + BAR_Q_FULL * 8, kTileBytes);
         for (int half = 0; half < 2; half++)
@@ -211,7 +212,7 @@ __device__ __forceinline__ void producer(const Ctx &c, const Params &p, const Ti
         for (int w = 0; w < 4; w++) {
             const int key = 32 * w + lane;
             bool valid = key < p.unit && row0 + key < p.seq_k;
-            if (valid && p.key_mask) valid = __ldg(p.key_mask + row0 + key) != 0;
+            if (valid && p.key_mask) valid = p.key_mask[row0 + key] != 0;
             const uint32_t b = __ballot_sync(0xffffffffu, valid);
             any |= b;
             /* Word of the tile that these keys belong to (two boxes of 16 keys share one). */
@@ -224,7 +225,7 @@ __device__ __forceinline__ void producer(const Ctx &c, const Params &p, const Ti
     };
 
     for (int e = t.e0; ok && e < t.e1; e += 32) {
-        if (e > t.e0) entry = e + lane < t.e1 ? __ldg(t.list + e + lane) : -1;
+        if (e > t.e0) entry = e + lane < t.e1 ? t.list[e + lane] : -1;
         unsigned todo = __ballot_sync(0xffffffffu, entry >= 0 && entry < p.k_blocks);
         while (ok && todo) {
             const int src = __ffs(todo) - 1;
@@ -424,8 +425,8 @@ __device__ __forceinline__ RowState softmax_rows(const Ctx &c, const Params &p, 
 }
 
 /* O times f -> bf16 rows, through 8 KB of staging per warp (two halves of 32
- * rows x 128 bytes, 16-byte chunks swizzled by the row): a thread owns a row, memory wants
- * eight threads per 128 bytes of it. */
+ * rows x 128 bytes, 16-byte chunks swizzled by the row): a thread owns a row,
+ * memory wants eight threads per 128 bytes of it. */
 __device__ __forceinline__ void store_rows(const Params &p, const Tile &t, uint32_t tmem, float f, bool any, unsigned char *stage) {
     const int row = threadIdx.x & 127, lane = threadIdx.x & 31, row0 = row & ~31;
     if (row0 >= t.rows) return;
@@ -498,8 +499,9 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
     /* The producer sets up the barriers and starts at once; it only tells the
      * other warps, which wait here for the barriers and the tensor memory. The
      * launch is stream-serialised by program: nothing may be read or written
-     * before the kernel ahead is complete, which the producer waits for and
-     * everything else follows from its loads. */
+     * before the kernel ahead is complete, and no bounded wait may have begun.
+     * (What is read may be written until then: no load through the
+     * non-coherent path, which takes memory as constant for the whole kernel.) */
     uint32_t tmem = 0;
     if (warp == 4) {
         if (lane == 0) {
@@ -510,7 +512,6 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
         }
         __syncwarp();
         asm volatile("barrier.cta.arrive.aligned 1, %0;" ::"n"(kThreads) : "memory");
-        asm volatile("griddepcontrol.wait;" ::: "memory");
     } else {
         if (warp == 5) {
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
@@ -522,6 +523,7 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
         tc_fence_after();
         tmem = *tmem_slot;
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     RowState st = {-INFINITY, 0.0f, false, true};
     if (warp < 4) {
@@ -621,7 +623,7 @@ bool attention_blocks_sm100_supported(const BlockAttnArgs &a) {
     const uintptr_t bits = (uintptr_t)a.out | (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v;
     const long long tiles = (long long)a.heads * a.q_blocks * (((a.q_block < a.seq_q ? a.q_block : a.seq_q) + 127) / 128);
     return a.head_dim == attn_blocks::kHeadDim && (a.k_block == 16 || a.k_block == 32 || a.k_block == 64 || a.k_block % 128 == 0) &&
-           a.ldo % 8 == 0 && a.ldq % 8 == 0 && a.ldk % 8 == 0 && a.ldv % 8 == 0 && (bits & 15) == 0 && a.seq_q > 0 && a.seq_k > 0 &&
+           a.ldo % 8 == 0 && a.ldq % 8 == 0 && a.ldk % 8 == 0 && a.ldv % 8 == 0 && (bits & 15) == 0 && a.seq_k > 0 &&
            tiles <= 0x7FFFFFFFll / attn_blocks::kMaxParts;
 }
 

@@ -20,6 +20,11 @@
  * the CTA that chooses for the row. One to eight warps then find the topk-th
  * largest key of a row by a search over its bits and write the chosen blocks
  * in ascending order, equal keys from the lowest index.
+ *
+ * Both kernels start under the kernel ahead of them and wait for its end. What
+ * they read may be written until then, so it is never read through the
+ * non-coherent path, which takes memory as constant for the whole kernel: no
+ * __ldg and no __restrict__ here.
  */
 #include "common.cuh"
 
@@ -40,8 +45,7 @@ static constexpr int kMeanRun = 8;               /* rows of a thread in flight, 
 /* VEC: 16-byte loads (head_dim and strides multiples of 8, aligned base). */
 template <bool VEC>
 __global__ void __launch_bounds__(kMeanThreads, 4)
-k_block_means(float *__restrict__ means, int *__restrict__ counts, const uint16_t *__restrict__ x, int ldx, int seq,
-              int width, int block, const int *__restrict__ row_mask) {
+k_block_means(float *means, int *counts, const uint16_t *x, int ldx, int seq, int width, int block, const int *row_mask) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ double part[8][kMeanCols];
     __shared__ int part_n[8];
@@ -54,10 +58,11 @@ k_block_means(float *__restrict__ means, int *__restrict__ counts, const uint16_
 #pragma unroll
     for (int i = 0; i < 8; i++) acc[i] = 0.0;
     int n = 0;
-    for (int rb = warp; rb < rows; rb += 8 * kMeanRun) {
+    /* (Unsigned: rb may pass the last row by more than a 31-bit count has room for.) */
+    for (unsigned rb = warp; rb < (unsigned)rows; rb += 8 * kMeanRun) {
         /* Which of the run's rows count (bit i: row rb + 8 i), then all their loads at once. */
-        const int mine = rb + 8 * lane;
-        const bool counts_mine = lane < kMeanRun && mine < rows && (!row_mask || __ldg(row_mask + r0 + mine) != 0);
+        const unsigned mine = rb + 8 * lane;
+        const bool counts_mine = lane < kMeanRun && mine < (unsigned)rows && (!row_mask || row_mask[r0 + mine] != 0);
         const unsigned ok = __ballot_sync(0xffffffffu, counts_mine);
         n += __popc(ok);
         uint4 v[kMeanRun];
@@ -67,7 +72,7 @@ k_block_means(float *__restrict__ means, int *__restrict__ counts, const uint16_
             if (!((ok >> i) & 1u)) continue;
             const uint16_t *src = x + (size_t)(r0 + rb + 8 * i) * ldx + c0;
             if (VEC) {
-                if (c0 < width) v[i] = __ldg(reinterpret_cast<const uint4 *>(src));
+                if (c0 < width) v[i] = *reinterpret_cast<const uint4 *>(src);
             } else {
                 uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
@@ -160,7 +165,7 @@ struct Block {
         row = krow;
 #pragma unroll
         for (int g = 0; g < HD / 16; g++)
-            v[g] = krow ? __ldg(reinterpret_cast<const float4 *>(krow + 16 * g + (lane & 3) * 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            v[g] = krow ? *reinterpret_cast<const float4 *>(krow + 16 * g + (lane & 3) * 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
 };
 
@@ -514,13 +519,13 @@ k_block_select(const __grid_constant__ Select p) {
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (HD > 0) {
             if (ok) {
-                const float4 f = __ldg(reinterpret_cast<const float4 *>(src));
+                const float4 f = *reinterpret_cast<const float4 *>(src);
                 v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
             }
         } else {
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                if (ok && e + k < p.head_dim) v[k] = __ldg(src + k);
+                if (ok && e + k < p.head_dim) v[k] = src[k];
         }
         double *dst = qf + (size_t)((row >> 3) * p.steps + (qd & ~3)) * 32 + (row & 7) * 4 + (qd & 3);
 #pragma unroll
@@ -537,7 +542,7 @@ k_block_select(const __grid_constant__ Select p) {
         for (int i = 0; i < 2; i++) {
             const int j = j0 + (lane & 3) * 2 + i;
             if (j >= b1) continue;
-            const bool ok = !p.counts || __ldg(p.counts + j) > 0;
+            const bool ok = !p.counts || p.counts[j] > 0;
             const bool kept = j < p.keep_first || j >= p.k_blocks - p.keep_last;
             for (int m = 0; m < tiles; m++) {
                 const int row = m * 8 + (lane >> 2);

@@ -77,12 +77,17 @@ __device__ __forceinline__ void turn_of(int p, Turn t, float &cs, float &sn) {
     sn = __uint_as_float(__float_as_uint(y) ^ (top & 0x80000000u));
 }
 
+/* Both 16-byte kernels start under the kernel ahead of them and wait for its
+ * end. What they read may be written until then, so it is never read through
+ * the non-coherent path, which takes memory as constant for the whole kernel:
+ * no __ldg and no __restrict__ here. */
+
 /* ---- tables ---- */
 
 /* A thread keeps VEC consecutive pairs for all its rows. */
 template <int VEC>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSM)
-k_rope_tables(float *__restrict__ cos_out, float *__restrict__ sin_out, const int *__restrict__ pos, int seq, int half,
+k_rope_tables(float *cos_out, float *sin_out, const int *pos, int seq, int half,
               const __grid_constant__ Plan plan) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int per_row = half / VEC, rows_per_block = kThreads / per_row;
@@ -105,7 +110,7 @@ k_rope_tables(float *__restrict__ cos_out, float *__restrict__ sin_out, const in
             const int *p = pos + row * plan.n;
             /* Neighbouring pairs mostly belong to one axis. */
 #pragma unroll
-            for (int i = 0; i < VEC; i++) at[k][i] = i > 0 && axis[i] == axis[i > 0 ? i - 1 : 0] ? at[k][i > 0 ? i - 1 : 0] : __ldg(p + axis[i]);
+            for (int i = 0; i < VEC; i++) at[k][i] = i > 0 && axis[i] == axis[i > 0 ? i - 1 : 0] ? at[k][i > 0 ? i - 1 : 0] : p[axis[i]];
         }
 #pragma unroll
         for (int k = 0; k < kTableRows; k++) {
@@ -206,7 +211,7 @@ k_qk_norm_rope_axes(const __grid_constant__ Rows a, const __grid_constant__ Plan
         {
             float c[PPL], s[PPL];
 #pragma unroll
-            for (int i = 0; i < PPL; i++) turn_of(__ldg(a.pos + (size_t)row * plan.n + axis[i]), turn[i], c[i], s[i]);
+            for (int i = 0; i < PPL; i++) turn_of(a.pos[(size_t)row * plan.n + axis[i]], turn[i], c[i], s[i]);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int src = (4 * l + i) / PPL;
@@ -218,8 +223,8 @@ k_qk_norm_rope_axes(const __grid_constant__ Rows a, const __grid_constant__ Plan
             /* Pair i of the lane is (x[i], x[4 + i]) with SPLIT, (x[2 i], x[2 i + 1]) without. */
             float k00[4], k01[4], k10[4], k11[4];
             if (NORM) {
-                const float4 w0 = __ldg(reinterpret_cast<const float4 *>(a.w[part] + d0));
-                const float4 w1 = __ldg(reinterpret_cast<const float4 *>(a.w[part] + d1));
+                const float4 w0 = *reinterpret_cast<const float4 *>(a.w[part] + d0);
+                const float4 w1 = *reinterpret_cast<const float4 *>(a.w[part] + d1);
                 const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {

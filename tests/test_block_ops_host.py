@@ -127,7 +127,7 @@ def test_attention_blocks_refusals(lib):
     for kw in (dict(out=None), dict(q=None), dict(k=None), dict(v=None), dict(lst=None), dict(ldo=511), dict(ldq=511),
                dict(ldk=255), dict(ldv=255), dict(sq=-1), dict(sk=-1), dict(heads=0), dict(kv=0), dict(kv=3), dict(hd=0), dict(scale=0.0),
                dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(n=-1), dict(qb=0), dict(kb=0), dict(kernel=3),
-               dict(kernel=-1)):
+               dict(kernel=-1), dict(n=2 ** 30 + 1), dict(heads=65536, kv=1, hd=1, ldo=65536, ldq=65536)):
         refused(lib, EINVAL, attn(**kw))
     refused(lib, EUNSUPPORTED, attn(hd=64, kernel=1))          # outside the tensor-core kernel's domain
     refused(lib, EUNSUPPORTED, attn(kb=48, kernel=1))

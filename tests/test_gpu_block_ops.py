@@ -295,6 +295,29 @@ def test_block_select_ties_go_to_the_lowest_block(lib):
     assert torch.equal(run_select(lib, one, same, None, 3, 0, 0), want)
 
 
+@pytest.mark.parametrize("nq,nk,kv", [(16, 100, 150), (16, 264, 150), (16, 500, 150), (16, 700, 150), (5, 300, 150), (2, 500, 150),
+                                      (1, 1100, 150), (2, 2000, 1), (1, 23552, 1), (16, 600, 1)])
+def test_block_select_many_equal_scores(lib, nq, nk, kv):
+    """Scores that are whole numbers between -8 and 8, so that hundreds of blocks are equal at the cut, over the sizes that
+    share a row between one, two, four and eight warps in one to eight CTAs."""
+    gen = torch.Generator().manual_seed(nk)
+    qm, km = torch.zeros(nq, kv, 128), torch.zeros(nk, kv, 128)
+    qm[..., ::16] = torch.randint(-1, 2, (nq, kv, 8), generator=gen).float()
+    km[..., ::16] = torch.randint(-1, 2, (nk, kv, 8), generator=gen).float()
+    counts = (torch.rand(nk, generator=gen) < 0.9).int()
+    first, last = 2, 3
+    score = torch.einsum("qhd,khd->hqk", qm.double(), km.double())
+    j = torch.arange(nk)
+    rank = score * nk - j                    # higher first, equal ones by the lowest block
+    rank = torch.where(((j < first) | (j >= nk - last)) & (counts > 0), rank + 100.0 * nk, rank)
+    rank = torch.where(counts > 0, rank, torch.full_like(rank, -100.0 * nk))
+    for topk in (5, nk // 3, nk - 1):
+        n = min(topk, int(counts.sum()))
+        want = torch.full((kv, nq, topk), -1, dtype=torch.int32)
+        want[..., :n] = rank.topk(n, dim=-1)[1].sort(-1)[0].int()
+        assert torch.equal(run_select(lib, qm, km, counts, topk, first, last), want)
+
+
 def test_block_select_values_that_are_not_finite(lib):
     qm, km = randn(1, 2, 1, 128), randn(2, 20, 1, 128)
     km[4] = NAN                              # ranks last, but before nothing
@@ -397,6 +420,12 @@ TENSOR = [  # sq, sk, heads, kv, list_len, q_block, k_block, masked, pad, junk
 def test_attention_tensor_kernel(lib, sq, sk, heads, kv, n, qb, kb, masked, pad, junk):
     check_attention(lib, sq, sk, heads, kv, 128, n, qb, kb, TCGEN05, masked, pad, junk)
     check_attention(lib, sq, sk, heads, kv, 128, n, qb, kb, TCGEN05, masked, pad, junk, seed=7, gain=3.0)
+
+
+@pytest.mark.parametrize("sq,heads,n,qb,masked,junk", [(2500, 30, 3, 128, False, False), (3700, 12, 35, 200, True, True),
+                                                       (11, 64, 5, 1, True, False)])
+def test_attention_tensor_kernel_more_tiles_than_fit_at_once(lib, sq, heads, n, qb, masked, junk):
+    check_attention(lib, sq, 2900, heads, 2, 128, n, qb, 64, TCGEN05, masked, 0, junk)
 
 
 @pytest.mark.parametrize("sq,heads,n", [(1, 8, 40), (300, 3, 6), (100, 2, 40)])
@@ -516,6 +545,85 @@ def test_the_operators_together(lib):
     a, b = out.double(), dense.cpu().double()
     mag = ref.attention(q.cpu(), k.cpu(), v.cpu(), heads, kv, D, D ** -0.5, mask, lists, qb, kb)[1]
     assert ((a - b).abs() <= 2.0 ** -7 * b.abs() + (2.0 ** -7 + 2.0 ** -11) * mag).all()
+
+
+def test_offsets_that_pass_32_bits(lib):
+    """Rows a long way apart: the last ones lie behind 2^31 elements of their tensor."""
+    seq, ld = 262400, 8320
+    x = torch.empty(seq, ld, dtype=torch.bfloat16, device="cuda")
+    rows = randn(1, seq, D).bfloat16().cuda()
+    x[:, :D] = rows
+    assert seq * ld > 2 ** 31 + 2 ** 25
+    means = torch.empty(seq // 64, D).cuda()
+    assert lib.iris_b200_block_means(ptr(means), None, ptr(x), ld, seq, 1, D, 64, None) == 0
+    done(lib)
+    assert (means.double() - rows.double().reshape(-1, 64, D).mean(1)).abs().max() < 1e-6
+    lists = torch.tensor([[[0, seq // 64 - 1, seq // 128]]], dtype=torch.int32)
+    keys = torch.cat([torch.arange(b * 64, b * 64 + 64) for b in lists[0, 0].tolist()])
+    q, kr = randn(2, 100, D).bfloat16(), rows[keys.cuda()].cpu()
+    want, mag = ref.attention(q, kr, kr, 1, 1, D, D ** -0.5, None, torch.tensor([[[0, 1, 2]]]), 100, 64)
+    dq, dl = q.cuda(), lists.cuda()
+    for kernel in (GENERIC, TCGEN05):
+        out = torch.zeros(100, D).bfloat16().cuda()
+        assert lib.iris_b200_attention_blocks(ptr(out), D, ptr(dq), D, ptr(x), ld, ptr(x), ld, 100, seq, 1, 1, D, D ** -0.5, None,
+                                              ptr(dl), 3, 100, 64, kernel) == 0
+        done(lib)
+        got = out.cpu().double()
+        assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * mag).all()
+    plan = lib.rope_axes((128,), None, 256.0, False, D)
+    pos = torch.zeros(seq, 1, dtype=torch.int32).cuda()        # no turn: rows come back as they are
+    x[:, D] = 0.0
+    for offset in (0, 1):                    # 16-byte kernel, general kernel
+        rows = x[:, offset:offset + D].clone()
+        assert lib.iris_b200_qk_norm_rope_axes(ptr(x, offset), ld, None, 0, ptr(x, offset), None, ld, None, None, ptr(pos), plan, seq, 1,
+                                               0, D, 0.0, 0) == 0
+        done(lib)
+        if offset == 0:
+            assert torch.equal(x[:, :D], rows)
+        else:
+            assert torch.equal(x[:, 1:D], rows[:, :-1])
+
+
+def test_calls_behind_one_another_see_what_the_last_one_wrote(lib):
+    """The launches overlap at their ends and reuse the same buffers: each has to read what the call before it wrote, not what
+    it may have read there one call earlier."""
+    heads, seq, qb, kb, topk = 8, 2048, 128, 64, 6
+    nq, nk = seq // qb, seq // kb
+    xs = [(randn(s, seq, heads * D) * (1.0 + s)).bfloat16().cuda() for s in range(3)]
+    poss = [positions(s, seq, 3, 900).cuda() for s in range(3)]
+    plan = lib.rope_axes((32, 48, 48), None, 256.0, False, D)
+    q, pos = torch.zeros(seq, heads * D).bfloat16().cuda(), torch.zeros(seq, 3, dtype=torch.int32).cuda()
+    qm, km = torch.zeros(nq, heads, D).cuda(), torch.zeros(nk, heads, D).cuda()
+    lists = torch.zeros(heads, nq, topk, dtype=torch.int32).cuda()
+
+    def step(i, out, kept, cos, sin):
+        pos.copy_(poss[i])
+        rc = lib.iris_b200_rope_axes_tables(ptr(cos), ptr(sin), ptr(pos), plan, seq, D)
+        rc |= lib.iris_b200_qk_norm_rope_axes(ptr(q), heads * D, None, 0, ptr(xs[i]), None, heads * D, None, None, ptr(pos), plan,
+                                              seq, heads, 0, D, 1e-6, 0)
+        rc |= lib.iris_b200_block_means(ptr(qm), None, ptr(q), heads * D, seq, heads, D, qb, None)
+        rc |= lib.iris_b200_block_means(ptr(km), None, ptr(q), heads * D, seq, heads, D, kb, None)
+        rc |= lib.iris_b200_block_select(ptr(lists), ptr(qm), ptr(km), None, nq, nk, heads, heads, D, topk, 0, 0)
+        rc |= lib.iris_b200_attention_blocks(ptr(out), heads * D, ptr(q), heads * D, ptr(q), heads * D, ptr(xs[i]), heads * D, seq, seq,
+                                             heads, heads, D, D ** -0.5, None, ptr(lists), topk, qb, kb, AUTO)
+        rc |= lib.iris_b200_block_select(ptr(kept), ptr(qm), ptr(km), None, nq, nk, heads, heads, D, topk, 0, 0)
+        assert rc == 0
+
+    def buffers():
+        return (torch.zeros(seq, heads * D).bfloat16().cuda(), torch.zeros_like(lists), torch.zeros(seq, D // 2).cuda(),
+                torch.zeros(seq, D // 2).cuda())
+
+    alone = []
+    for i in range(3):
+        alone.append(buffers())
+        step(i, *alone[i])
+        done(lib)
+    runs = [buffers() for _ in range(30)]
+    for n, b in enumerate(runs):
+        step(n % 3, *b)
+    done(lib)
+    for n, b in enumerate(runs):
+        assert all(torch.equal(x, y) for x, y in zip(b, alone[n % 3])), n
 
 
 def test_captured_and_replayed(lib):
