@@ -187,5 +187,6 @@ extern "C" int iris_b200_attention_blocks(uint16_t *out, int ldo, const uint16_t
     }
     if (!require_device(op)) return IRIS_B200_ENODEV;
     if (seq_q == 0) return IRIS_B200_OK;
+    if (kernel == IRIS_B200_KERNEL_AUTO && attention_blocks_row_supported(a)) return launch_attention_blocks_row(a);
     return fast && kernel != IRIS_B200_KERNEL_GENERIC ? launch_attention_blocks_sm100(a) : launch_any(a);
 }

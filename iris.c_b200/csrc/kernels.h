@@ -202,6 +202,9 @@ struct BlockAttnArgs {
 /* Whether the tensor-core kernel takes these arguments, and its launch. */
 bool attention_blocks_sm100_supported(const BlockAttnArgs &a);
 int launch_attention_blocks_sm100(const BlockAttnArgs &a);
+/* The same of the kernel for rows with a list of their own. */
+bool attention_blocks_row_supported(const BlockAttnArgs &a);
+int launch_attention_blocks_row(const BlockAttnArgs &a);
 /* Per-device launch configuration is redone after a cleanup. */
 void block_select_release(void);
 void attention_blocks_release(void);

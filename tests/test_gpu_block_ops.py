@@ -422,6 +422,42 @@ def test_attention_tensor_kernel(lib, sq, sk, heads, kv, n, qb, kb, masked, pad,
     check_attention(lib, sq, sk, heads, kv, 128, n, qb, kb, TCGEN05, masked, pad, junk, seed=7, gain=3.0)
 
 
+ROWS = [  # sq, sk, heads, kv, hd, list_len, k_block, masked, pad, junk
+    (1, 1, 1, 1, 128, 1, 1, False, 0, False), (1, 9, 2, 1, 64, 3, 7, False, 0, True), (5, 333, 3, 3, 256, 9, 16, True, 8, True),
+    (3, 4096, 4, 1, 128, 64, 64, True, 0, True), (1, 4096, 8, 2, 128, 40, 64, False, 0, False), (1, 2000, 2, 2, 64, 2, 900, True, 0, False),
+    (40, 700, 12, 4, 128, 5, 48, True, 16, True), (2, 9000, 1, 1, 256, 33, 33, True, 0, False), (1, 5000, 1, 1, 128, 300, 16, True, 0, True),
+    (300, 1000, 2, 2, 64, 17, 32, True, 0, True)]
+
+
+@pytest.mark.parametrize("sq,sk,heads,kv,hd,n,kb,masked,pad,junk", ROWS)
+def test_attention_row_kernel(lib, sq, sk, heads, kv, hd, n, kb, masked, pad, junk):
+    check_attention(lib, sq, sk, heads, kv, hd, n, 1, kb, AUTO, masked, pad, junk)
+    check_attention(lib, sq, sk, heads, kv, hd, n, 1, kb, AUTO, masked, pad, junk, seed=7, gain=3.0)
+    if sq == 1:                              # the only query, whatever its block is called
+        check_attention(lib, sq, sk, heads, kv, hd, n, 100, kb, AUTO, masked, pad, junk)
+
+
+def test_attention_row_kernel_without_keys_and_not_finite(lib):
+    q, k, v = (randn(i, r, 256).bfloat16() for i, r in enumerate((4, 200, 200)))
+    mask = torch.ones(200, dtype=torch.int32)
+    mask[64:128] = 0                          # block 1 is masked as a whole
+    v[70:90], k[100] = NAN, NAN               # and holds no numbers
+    v[10, 5], k[140] = NAN, NAN               # seen by the lists that hold blocks 0 and 2
+    lists = torch.tensor([[[-1, -1, -1], [9, -5, 4], [1, -1, 1], [3, -1, 1]], [[0, 3, 1], [2, 2, -1], [3, 3, 9], [1, 9, 3]]], dtype=torch.int32)
+    got = run_attention(lib, q, k, v, 2, 2, 128, mask, lists, 1, 64, AUTO)
+    bad = got.isnan()
+    assert (got[:3, :128] == 0).all() and not bad[3].any() and not bad[2].any()
+    assert not bad[0, 128:].any() and bad[1, 128:].all()         # column 5 of row 10 is head 0's
+    got = run_attention(lib, q, k, v, 2, 2, 128, mask, lists.flip(0), 1, 64, AUTO)
+    assert got[0, :128].isnan().sum() == 1 and got[0, 5].isnan()
+    want, _ = ref.attention(q[2:], k[:140], v[:140], 2, 2, 128, 128 ** -0.5, mask[:140], torch.full((2, 2, 1), 0), 1, 8)
+    got = run_attention(lib, q[2:], k[:140], v[:140], 2, 2, 128, mask[:140], torch.full((2, 2, 1), 0, dtype=torch.int32), 1, 8, AUTO)
+    assert (got - want).abs().max() < 0.05
+    for sk, n in ((0, 2), (200, 0)):
+        got = run_attention(lib, q, k[:sk], v[:sk], 2, 2, 128, None, torch.zeros(2, 4, n, dtype=torch.int32), 1, 64, AUTO)
+        assert (got == 0).all()
+
+
 @pytest.mark.parametrize("sq,heads,n,qb,masked,junk", [(2500, 30, 3, 128, False, False), (3700, 12, 35, 200, True, True),
                                                        (11, 64, 5, 1, True, False)])
 def test_attention_tensor_kernel_more_tiles_than_fit_at_once(lib, sq, heads, n, qb, masked, junk):
@@ -479,9 +515,10 @@ def test_attention_rows_without_keys(lib, kernel):
 def test_attention_block_listed_twice_counts_twice(lib, kernel):
     q, k, v = (randn(20 + i, r, 128).bfloat16() for i, r in enumerate((50, 256, 256)))
     lists = torch.tensor([[[1, 3, 1, -1]]], dtype=torch.int32)
-    got = run_attention(lib, q, k, v, 1, 1, 128, None, lists, 50, 64, kernel)
-    want, mag = ref.attention(q, k, v, 1, 1, 128, 128 ** -0.5, None, lists, 50, 64)
-    assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * mag).all()
+    for rows in (50, 1):
+        got = run_attention(lib, q[:rows], k, v, 1, 1, 128, None, lists, 50, 64, kernel)
+        want, mag = ref.attention(q[:rows], k, v, 1, 1, 128, 128 ** -0.5, None, lists, 50, 64)
+        assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * mag).all()
 
 
 # ---------------------------------------------------------------------------
