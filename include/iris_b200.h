@@ -451,7 +451,10 @@ int iris_b200_block_select(int *list, const float *q_means, const float *k_means
  * list_len <= 2^30, heads <= 65535. kernel: one of IRIS_B200_KERNEL_*; the
  * tcgen05 kernel serves head_dim 128, k_block 16, 32, 64 or a multiple of 128,
  * strides in multiples of 8 and 16-byte aligned pointers, the general one
- * everything up to head_dim 512. */
+ * everything up to head_dim 512. The automatic choice has a third kernel for
+ * q_block 1 or a single query row (tokens at the end of a long cache), with
+ * head_dim 64, 128 or 256, any k_block, the same strides and alignment of q, k
+ * and v. */
 int iris_b200_attention_blocks(uint16_t *out, int ldo, const uint16_t *q, int ldq,
                                const uint16_t *k, int ldk, const uint16_t *v, int ldv,
                                int seq_q, int seq_k, int heads, int kv_heads, int head_dim, float scale,

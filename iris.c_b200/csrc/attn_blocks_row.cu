@@ -13,8 +13,17 @@
  *
  * Maximum, sum and accumulators are fp32 and private to a warp; probabilities
  * are not rounded. The chunks of a list go round the warps of a cluster of up
- * to eight CTAs, whose results meet in shared memory: first in each CTA, then
- * in the first one.
+ * to sixteen CTAs, whose results meet in shared memory: first in each CTA,
+ * then in the first one.
+ *
+ * Bound by HBM where the lists of a call do not fit in L2: one row of 32 heads
+ * over 64 blocks of 64 keys each, 67 MB, takes 14.7 us back to back (4.6 TB/s);
+ * with head_dim 256, 134 MB, 24.4 us, so that 67 MB more cost 9.6 us (7.0
+ * TB/s) and 5 us are launch, list, first loads and joining. The tensor-core
+ * kernel takes 19.1 us for the former, and for 256 rows of 32 heads over 32
+ * blocks, out of L2, 893 us against 712. Half as many loads per warp and twice
+ * the warps: 20.8 us; the next chunk's loads started under the products of
+ * this one, which spills: 15.0 us and 856 us.
  */
 #include "common.cuh"
 
@@ -32,7 +41,7 @@ using namespace sm100;
 static constexpr int kThreads = 256;
 static constexpr int kWarps = kThreads / 32;
 static constexpr int kCtasPerSM = 2;
-static constexpr int kMaxParts = 8;
+static constexpr int kMaxParts = 16;              /* CTAs of a cluster, where the device takes as many */
 static constexpr int kLoads = 8;                 /* K rows of a lane in flight, and as many V rows */
 
 struct Params {
@@ -239,6 +248,34 @@ k_attention_blocks_row(const __grid_constant__ Params p) {
     cluster_sync_all();                          /* nobody leaves while its sums are being read */
 }
 
+static int g_max_parts = 0;                      /* 0: not asked yet */
+
+/* Sixteen CTAs are more than every device promises a cluster: 1 head over 128
+ * blocks of 64 keys takes 7.9 us so, 12.0 us with eight; 8 heads over 64 blocks
+ * 7.7 and 9.3 us. */
+static int max_parts() {
+    if (g_max_parts) return g_max_parts;
+    auto allow = [](auto kernel) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+    };
+    int parts = 8;
+    if (allow(k_attention_blocks_row<64>) && allow(k_attention_blocks_row<128>) && allow(k_attention_blocks_row<256>)) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(kMaxParts);
+        cfg.blockDim = dim3(kThreads);
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = kMaxParts;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int fit = 0;
+        if (cudaOccupancyMaxActiveClusters(&fit, k_attention_blocks_row<256>, &cfg) == cudaSuccess && fit > 0) parts = kMaxParts;
+    }
+    if (parts < kMaxParts) (void)cudaGetLastError();     /* a refusal here is an answer, not an error */
+    return g_max_parts = parts;
+}
+
 /* Keys of a chunk. */
 static int chunk_keys(int head_dim) { return kLoads * 32 / (head_dim / 8); }
 
@@ -249,11 +286,13 @@ static long long chunks_of(const BlockAttnArgs &a) {
 
 }  // namespace attn_row
 
+void attention_blocks_row_release(void) { attn_row::g_max_parts = 0; }
+
 bool attention_blocks_row_supported(const BlockAttnArgs &a) {
     const uintptr_t bits = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v;
     return (a.q_block == 1 || a.seq_q == 1) && (a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) && a.ldq % 8 == 0 &&
            a.ldk % 8 == 0 && a.ldv % 8 == 0 && (bits & 15) == 0 && a.seq_k > 0 && a.seq_q <= INT_MAX / attn_row::kMaxParts &&
-           attn_row::chunks_of(a) <= INT_MAX - 64 * 32;
+           attn_row::chunks_of(a) <= INT_MAX - 32 * attn_row::kMaxParts * attn_row::kWarps;
 }
 
 int launch_attention_blocks_row(const BlockAttnArgs &a) {
@@ -263,11 +302,11 @@ int launch_attention_blocks_row(const BlockAttnArgs &a) {
     p.chunks = (int)chunks_of(a);
     p.chunks_per_entry = a.list_len > 0 ? p.chunks / a.list_len : 1;
     p.scale_log2 = a.scale * 1.4426950408889634f;
-    /* The list of a row is cut over the CTAs of a cluster while that leaves room
-     * on the device otherwise and every warp keeps a chunk. */
+    /* The list of a row is cut over the CTAs of a cluster while the device has
+     * room for more and every warp keeps a chunk. */
     const long long items = (long long)a.heads * a.seq_q;
     p.parts = 1;
-    while (p.parts < kMaxParts && items * p.parts * 2 <= (long long)kCtasPerSM * g.sm_count && p.chunks >= p.parts * 2 * kWarps) p.parts *= 2;
+    while (p.parts < max_parts() && items * p.parts * 2 <= (long long)kCtasPerSM * g.sm_count && p.chunks >= p.parts * 2 * kWarps) p.parts *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.seq_q * p.parts), (unsigned)a.heads);
     cfg.blockDim = dim3(kThreads);

@@ -208,6 +208,7 @@ int launch_attention_blocks_row(const BlockAttnArgs &a);
 /* Per-device launch configuration is redone after a cleanup. */
 void block_select_release(void);
 void attention_blocks_release(void);
+void attention_blocks_row_release(void);
 
 /* Shared argument checks of the device-pointer attention entry points. */
 int check_attention_args(const char *op, const void *out, const void *q, const void *k, const void *v, int ldo,

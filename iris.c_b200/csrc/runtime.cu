@@ -138,6 +138,7 @@ void iris_dev_cleanup(void) {
     sm100_release();
     block_select_release();
     attention_blocks_release();
+    attention_blocks_row_release();
     if (g.scratch) cuda_ok(cudaFree(g.scratch), "free");
     g.scratch = NULL;
     g.scratch_bytes = 0;
