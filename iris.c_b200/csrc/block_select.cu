@@ -115,7 +115,8 @@ k_block_means(float *means, int *counts, const uint16_t *x, int ldx, int seq, in
 static constexpr int kSelThreads = 256;
 static constexpr int kSelWarps = kSelThreads / 32;
 static constexpr int kSelRows = 16;              /* (query block, head) rows of a cluster: two score tiles of eight */
-static constexpr int kMaxCtas = 8;               /* CTAs of a cluster, each with a slice of the blocks */
+static constexpr int kMaxCtas = 16;              /* CTAs of a cluster, each with a slice of the blocks */
+static constexpr int kWideSmem = 96 * 1024;      /* of a CTA in a cluster of more than eight: two CTAs fit an SM */
 static constexpr int kMaxBlocks = 23552;         /* 64-bit keys of one row in shared memory */
 static constexpr int kMaxHeadDim = 512;
 static constexpr int kSelSmem = kMaxBlocks * 8 + kMaxHeadDim * 64;      /* one row's keys, one tile of rows */
@@ -584,6 +585,32 @@ k_block_select(const __grid_constant__ Select p) {
 }
 
 static int g_select_ready = 0;
+static int g_max_ctas = 8;
+
+/* Sixteen CTAs are more than every device promises a cluster (4 rows of 8 key
+ * heads over 2048 blocks: 12.4 us so, 13.8 us with eight). */
+static bool wide_clusters() {
+    auto allow = [](auto kernel) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+    };
+    bool ok = allow(k_block_select<128>) && allow(k_block_select<64>) && allow(k_block_select<0>);
+    if (ok) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(kMaxCtas);
+        cfg.blockDim = dim3(kSelThreads);
+        cfg.dynamicSmemBytes = kWideSmem;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = kMaxCtas;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int fit = 0;
+        ok = cudaOccupancyMaxActiveClusters(&fit, k_block_select<128>, &cfg) == cudaSuccess && fit > 0;
+    }
+    if (!ok) (void)cudaGetLastError();           /* a refusal here is an answer, not an error */
+    return ok;
+}
 
 static int bad(const char *op, const char *why) {
     set_error(IRIS_B200_EINVAL, op, why);
@@ -667,31 +694,33 @@ extern "C" int iris_b200_block_select(int *list, const float *q_means, const flo
     p.keep_first = keep_first < k_blocks ? keep_first : k_blocks;
     p.keep_last = keep_last < k_blocks ? keep_last : k_blocks;
     p.steps = (head_dim + 15) / 16 * 4;
+    if (!g_select_ready) {
+        if (!cuda_ok(cudaFuncSetAttribute(k_block_select<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem), op) ||
+            !cuda_ok(cudaFuncSetAttribute(k_block_select<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem), op) ||
+            !cuda_ok(cudaFuncSetAttribute(k_block_select<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem), op))
+            return IRIS_B200_ECUDA;
+        g_max_ctas = wide_clusters() ? kMaxCtas : 8;
+        g_select_ready = 1;
+    }
     /* Rows of a cluster: as many as there are, up to two score tiles, and as
-     * the keys of fit in shared memory. The blocks are cut over a cluster while
+     * fit in shared memory with their keys. The blocks are cut over a cluster while
      * that leaves SMs idle otherwise (two CTAs per SM), down to one tile of
      * eight blocks per warp. */
     const long long rows = (long long)q_blocks * p.group;
     p.rows = rows < kSelRows ? (int)rows : kSelRows;
     auto tiles_of = [&] { return (rows + p.rows - 1) / p.rows; };
     p.ctas = 1;
-    while (p.ctas < kMaxCtas && tiles_of() * kv_heads * p.ctas * 2 <= 2LL * g.sm_count && k_blocks >= p.ctas * 2 * kSelWarps * 8)
-        p.ctas *= 2;
     auto smem_of = [&] {
         p.own_rows = (p.rows + p.ctas - 1) / p.ctas;
         return (size_t)(p.rows > 8 ? 2 : 1) * p.steps * 256 + (size_t)p.own_rows * k_blocks * 8;
     };
+    while (p.ctas < g_max_ctas && tiles_of() * kv_heads * p.ctas * 2 <= 2LL * g.sm_count && k_blocks >= p.ctas * 2 * kSelWarps * 8)
+        p.ctas *= 2;
+    if (p.ctas > 8 && smem_of() > kWideSmem) p.ctas = 8;
     while (p.rows > 1 && smem_of() > kSelSmem) p.rows--;
     const size_t smem = smem_of();
     p.slice = ((k_blocks + p.ctas - 1) / p.ctas + 7) / 8 * 8;
     p.team = p.own_rows >= kSelWarps ? 1 : p.own_rows > 2 ? 2 : p.own_rows > 1 ? 4 : 8;
-    if (!g_select_ready) {
-        if (!cuda_ok(cudaFuncSetAttribute(k_block_select<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem), op) ||
-            !cuda_ok(cudaFuncSetAttribute(k_block_select<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem), op) ||
-            !cuda_ok(cudaFuncSetAttribute(k_block_select<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem), op))
-            return IRIS_B200_ECUDA;
-        g_select_ready = 1;
-    }
     const long long clusters = tiles_of();
     if (clusters * p.ctas > INT_MAX) return bad(op, "too many query blocks");
     cudaLaunchConfig_t cfg = {};
