@@ -63,7 +63,7 @@ static constexpr int kSmemK = kTileBytes;                /* K and V; later: a cl
 static constexpr int kSmemV = 2 * kTileBytes;
 static constexpr int kSmemBar = 3 * kTileBytes;
 static constexpr float kRescaleThreshold = 8.0f;
-static constexpr int kRegsSoftmax = 200, kRegsOther = 56;    /* 128 * 200 + 128 * 56 = the launch's 256 * 128 */
+static constexpr int kRegsSoftmax = 184, kRegsOther = 72;    /* 128 * 184 + 128 * 72 = the launch's 256 * 128 */
 static constexpr int kMaxParts = 8;
 static constexpr unsigned long long kDrainNs = 100000000ull;      /* for work in flight, beyond the wait limit */
 static constexpr int kMetaSlots = 4;
