@@ -4,15 +4,17 @@
  * thread per query row. head_dim 128.
  *
  * Work decomposition
- *   A CTA takes one tile of up to 128 rows of a query block of one head. Two
- *   CTAs share an SM (half of its tensor memory and shared memory each), so
- *   that the tensor pipe works for one while the other is in its softmax; the
- *   dense kernel pairs two tiles in one CTA instead, which needs both to walk
- *   the same keys. The CTAs are not persistent: there is no work list to keep
- *   between launches, and neighbouring CTAs take neighbouring tiles of one
- *   head, so that its K and V stay in L2. Where the tiles do not fill the
- *   device the list of a tile is cut over the CTAs of a cluster, which merge
- *   their results through distributed shared memory.
+ *   A CTA takes tiles of up to 128 rows of a query block of one head, one after
+ *   the other. Two CTAs share an SM (half of its tensor memory and shared
+ *   memory each), so that the tensor pipe works for one while the other is in
+ *   its softmax; the dense kernel pairs two tiles in one CTA instead, which
+ *   needs both to walk the same keys. The tiles go round the CTAs in order:
+ *   those in flight belong to few heads, whose K and V stay in L2, and Q, the
+ *   list, K and V of the next tile are on their way while the last one's
+ *   softmax, product and store finish (4333 rows x 30 heads over 18 blocks of
+ *   64 keys: 94 us with a CTA per tile, 86 us so). Where the tiles do not fill
+ *   the device the list of a tile is cut over the CTAs of a cluster, which
+ *   merge their results through distributed shared memory.
  *
  * Keys
  *   A key tile is 128 rows made of 128 / k_block listed blocks (or a piece of
@@ -22,13 +24,14 @@
  *   key: zero for rows behind seq_k, masked rows and the rows of a last tile
  *   that no block filled. Their scores become -inf whatever K holds; their V
  *   rows are cleared in shared memory before the MMA, since a zero probability
- *   does not cancel a NaN.
+ *   does not cancel a NaN. The mask is read one key tile ahead.
  *
  * Warps (256 threads)
- *   0-3  softmax: thread r owns row r of S / P / O
- *   4    producer
- *   5    MMA issuer, owner of the TMEM allocation
- *   6-7  idle: they complete the warpgroup that gives registers to the first
+ *   0-3      softmax: thread r owns row r of S / P / O
+ *   4 or 6   producer (6 in the second half of the CTAs, so that the two on an
+ *            SM, one of either half, do not share a scheduler)
+ *   5 or 7   MMA issuer, owner of the TMEM allocation
+ *   others   idle: they complete the warpgroup that gives registers to the first
  *
  * Tensor memory (256 columns): S [0, 128), O [128, 256); P (bf16) over the
  * front of S. MMA order: QK(0) PV(0) QK(1) PV(1) ...; each PV in two halves of
@@ -36,6 +39,18 @@
  * kernel: base 2, the reference value of a row moves only when its maximum
  * grows by more than 8, P rounded to bf16 for the MMA while the row sum keeps
  * fp32. A row without any key yields zeros.
+ *
+ * Records: the producer hands the tiles of keys and the end of every query
+ * tile to the softmax and MMA warps through a ring of four records, which all
+ * of them free again. Buffers of Q, K, V, S / P and O are single; barrier
+ * parities count key tiles (Q, O: query tiles with keys) of the whole CTA.
+ *
+ * Bound by the chain scores -> softmax -> product: 16 896 rows x 32 heads over
+ * 64 blocks of 64 keys take 1 010 to 1 040 us (1.09 to 1.12 PFLOP/s), where the
+ * products alone would take 690. Per pair of key tiles an SM spends about 3 700
+ * cycles, 2 048 of them in products and, beside them, 2 048 in exponentials;
+ * the two CTAs alternate, a softmax takes 1 700 cycles and the way from its
+ * last probability to its next scores 1 400.
  *
  * Every wait on a barrier is bounded as in the dense kernel; a CTA that gives
  * up still takes part in the cluster's barriers.
@@ -58,10 +73,11 @@ static constexpr int kHeadDim = 128;
 static constexpr int kTile = 128;                        /* query rows / keys of a tile */
 static constexpr int kHalfBytes = 128 * 64 * 2;          /* one [128 x 64] bf16 swizzled operand half */
 static constexpr int kTileBytes = 2 * kHalfBytes;
-static constexpr int kSmemQ = 0;                         /* later: staging of the output rows */
+static constexpr int kSmemQ = 0;
 static constexpr int kSmemK = kTileBytes;                /* K and V; later: a cluster's partial rows */
 static constexpr int kSmemV = 2 * kTileBytes;
-static constexpr int kSmemBar = 3 * kTileBytes;
+static constexpr int kSmemStage = 3 * kTileBytes;        /* output rows, 4 KB per softmax warp; or a cluster's (maximum, sum) */
+static constexpr int kSmemBar = kSmemStage + 4 * 4096;
 static constexpr float kRescaleThreshold = 8.0f;
 static constexpr int kRegsSoftmax = 184, kRegsOther = 72;    /* 128 * 184 + 128 * 72 = the launch's 256 * 128 */
 static constexpr int kMaxParts = 8;
@@ -79,20 +95,25 @@ enum {
     BAR_P_FULL,                         /* 2: halves of the key tile */
     BAR_O_DONE = BAR_P_FULL + 2,
     BAR_DRAIN,
-    BAR_META,                           /* kMetaSlots */
-    BAR_COUNT = BAR_META + kMetaSlots
+    BAR_META,                           /* kMetaSlots: a record is there */
+    BAR_META_FREE = BAR_META + kMetaSlots,      /* kMetaSlots: its readers, four softmax warps and the MMA warp, are through */
+    BAR_COUNT = BAR_META_FREE + kMetaSlots
 };
 static constexpr int kOffTmemPtr = BAR_COUNT * 8;
 static constexpr int kOffAbort = kOffTmemPtr + 4;
-static constexpr int kOffMeta = 128;                     /* kMetaSlots x 32 bytes */
-static constexpr int kOffMl = 256;                       /* 128 x (maximum, sum) */
-static constexpr int kSmemBytes = kSmemBar + kOffMl + 128 * 8;
-static_assert(kOffAbort + 4 <= kOffMeta && kOffMeta + kMetaSlots * 32 <= kOffMl, "barrier block");
+static constexpr int kOffMeta = 160;                     /* kMetaSlots x 32 bytes */
+static constexpr int kSmemBytes = kSmemBar + kOffMeta + kMetaSlots * 32;
+static_assert(kOffAbort + 4 <= kOffMeta, "barrier block");
+static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
 
-/* What the producer publishes with a key tile. */
+/* What the producer publishes: the key tiles of a query tile, and its end. */
+static constexpr uint32_t kEnd = 0, kEndUnused = 4;      /* unused: Q was loaded, but there was no key tile */
+static constexpr uint32_t kWhole = 1, kPartly = 2;       /* a key tile with all keys valid, with invalid keys */
+__device__ __forceinline__ bool is_end(uint32_t state) { return (state & 3u) == kEnd; }
+
 struct Meta {
     uint32_t bits[4];                   /* valid keys */
-    uint32_t state;                     /* 1: a tile, all keys valid; 2: a tile with invalid keys; 0: the end */
+    uint32_t state;                     /* kEnd, kEndUnused, kWhole or kPartly */
     uint32_t pad[3];
 };
 
@@ -103,8 +124,8 @@ struct Params {
     const int *key_mask;
     const int *list;
     int list_len, q_block, q_blocks, k_block, k_blocks;
-    int tiles;                          /* query tiles of a query block */
-    int unit, units, per_entry;         /* rows of a TMA box, boxes of a tile, boxes of a list entry */
+    int tiles, per_head, items;         /* query tiles of a query block, of a head, of the launch */
+    int unit, unit_log, units, per_entry;       /* rows of a TMA box, boxes of a tile, boxes of a list entry */
     int parts, part_len;                /* CTAs of a cluster, list entries of each */
     float scale_log2;
     unsigned int *status;
@@ -135,10 +156,10 @@ struct Tile {
     const int *list;
     int e0, e1;                         /* this CTA's entries */
 };
-__device__ __forceinline__ Tile tile_of(const Params &p, int rank) {
+__device__ __forceinline__ Tile tile_of(const Params &p, int item, int rank) {
     Tile t;
-    t.head = (int)blockIdx.y;
-    const int in_head = p.parts > 1 ? (int)(blockIdx.x / (unsigned)p.parts) : (int)blockIdx.x;
+    t.head = item / p.per_head;
+    const int in_head = item - t.head * p.per_head;
     const int qb = p.tiles > 1 ? in_head / p.tiles : in_head, in_block = (in_head - qb * p.tiles) * kTile;
     t.q0 = qb * p.q_block + in_block;
     int rows = p.q_block - in_block < kTile ? p.q_block - in_block : kTile;
@@ -150,48 +171,60 @@ __device__ __forceinline__ Tile tile_of(const Params &p, int rank) {
     if (rows <= 0) t.e1 = t.e0;
     return t;
 }
+/* A CTA's query tiles: first_item, + item_step, ... below p.items. (A cluster has one.) */
+__device__ __forceinline__ int first_item(const Params &p) { return p.parts > 1 ? (int)(blockIdx.x / (unsigned)p.parts) : (int)blockIdx.x; }
+__device__ __forceinline__ int item_step(const Params &p) { return p.parts > 1 ? p.items : (int)gridDim.x; }
 
-__device__ __forceinline__ void producer(const Ctx &c, const Params &p, const Tile &t, const CUtensorMap *mq, const CUtensorMap *mk,
+__device__ __forceinline__ void producer(const Ctx &c, const Params &p, int rank, const CUtensorMap *mq, const CUtensorMap *mk,
                                          const CUtensorMap *mv, uint32_t smem, volatile Meta *meta, int lane) {
-    const int qcol = t.head * kHeadDim, kcol = (t.head / p.group) * kHeadDim;
-    int j = 0;                          /* tiles published */
-    int loads_k = 0, loads_v = 0;       /* tiles whose K / V copies were started */
-    /* Q and the first entries of the list are on their way before anything else. */
-    int entry = t.e0 + lane < t.e1 ? t.list[t.e0 + lane] : -1;
-    if (lane == 0 && t.e0 < t.e1) {
-        mbar_expect_tx(c.bars + BAR_Q_FULL * 8, kTileBytes);
-        for (int half = 0; half < 2; half++)
-            tma_load_2d(smem + kSmemQ + half * kHalfBytes, mq, qcol + half * 64, t.q0, c.bars + BAR_Q_FULL * 8);
-    }
-    __syncwarp();
-    int filled = 0;                     /* boxes of the tile being put together; lane u holds the first row of box u */
+    int r = 0, j = 0;                   /* records published, key tiles loaded */
+    int loads_q = 0, loads_v = 0;
+    int filled = 0;                     /* boxes of the key tile being put together; lane u holds the first row of box u */
     int row_of_unit = 0;
     uint32_t key_bits = 0;              /* lane w: valid keys [32 w, 32 w + 32) of the tile */
-    bool ok = true;
+    bool ok = true, unused = false;     /* unused: Q is loaded, no key tile of it yet */
+    int kcol = 0;
 
-    /* Publish (and load) the tile at hand; the end of the list when it is empty. */
-    auto emit = [&]() -> bool {
-        const int n = filled;
-        const uint32_t par = (uint32_t)(j - 1) & 1u;
-        /* QK(j - 1) is done: K's buffer is free, and every reader is through with the tile record of four tiles ago. */
-        if (j > 0 && !__all_sync(0xffffffffu, wait_bar(c, BAR_K_EMPTY, par, 400))) return false;
-        volatile Meta *m = meta + (j & (kMetaSlots - 1));
+    auto load_q = [&](const Tile &t) {
+        unused = t.e0 < t.e1;
+        if (!unused) return;
+        if (lane == 0) {
+            mbar_expect_tx(c.bars + BAR_Q_FULL * 8, kTileBytes);
+            for (int half = 0; half < 2; half++)
+                tma_load_2d(smem + kSmemQ + half * kHalfBytes, mq, t.head * kHeadDim + half * 64, t.q0, c.bars + BAR_Q_FULL * 8);
+        }
+        __syncwarp();
+        loads_q++;
+    };
+
+    /* Publish (and load) the key tile at hand, or the end of the query tile. */
+    auto emit = [&](bool end) -> bool {
+        const int slot = r & (kMetaSlots - 1);
+        if (r >= kMetaSlots && !__all_sync(0xffffffffu, wait_bar(c, BAR_META_FREE + slot, (uint32_t)(r / kMetaSlots - 1) & 1u, 403)))
+            return false;
+        volatile Meta *m = meta + slot;
         const bool whole = __all_sync(0xffffffffu, lane >= 4 || key_bits == 0xFFFFFFFFu);
         if (lane < 4) m->bits[lane] = key_bits;
         key_bits = 0;
-        if (lane == 0) m->state = n == 0 ? 0u : whole ? 1u : 2u;
+        if (lane == 0) m->state = end ? (unused ? kEndUnused : kEnd) : whole ? kWhole : kPartly;
         __syncwarp();
-        if (lane == 0) mbar_arrive(c.bars + (BAR_META + (j & (kMetaSlots - 1))) * 8);
-        if (n == 0) return true;
-        const uint32_t bytes = (uint32_t)(n * p.unit * 256);
+        if (lane == 0) mbar_arrive(c.bars + (BAR_META + slot) * 8);
+        r++;
+        if (end) return true;
+        const int n = filled;
+        const uint32_t bytes = (uint32_t)(n * p.unit * 256), par = (uint32_t)(j - 1) & 1u;
+        if (j > 0 && !__all_sync(0xffffffffu, wait_bar(c, BAR_K_EMPTY, par, 400))) return false;       /* QK(j - 1) is done */
         if (lane == 0) mbar_expect_tx(c.bars + BAR_K_FULL * 8, bytes);
+        unused = false;
         __syncwarp();
         if (lane < n)
             for (int half = 0; half < 2; half++)
                 tma_load_2d(smem + kSmemK + half * kHalfBytes + lane * p.unit * 128, mk, kcol + half * 64, row_of_unit,
                             c.bars + BAR_K_FULL * 8);
-        loads_k++;
-        if (j > 0 && !__all_sync(0xffffffffu, wait_bar(c, BAR_V_EMPTY, par, 401))) return false;
+        __syncwarp();
+        j++;
+        filled = 0;
+        if (j > 1 && !__all_sync(0xffffffffu, wait_bar(c, BAR_V_EMPTY, par, 401))) return false;
         if (lane == 0) mbar_expect_tx(c.bars + BAR_V_FULL * 8, bytes);
         __syncwarp();
         if (lane < n)
@@ -200,66 +233,156 @@ __device__ __forceinline__ void producer(const Ctx &c, const Params &p, const Ti
                             c.bars + BAR_V_FULL * 8);
         __syncwarp();
         loads_v++;
-        j++;
-        filled = 0;
         return true;
     };
 
-    /* One box of rows joins the tile at hand, unless the mask leaves none of them. */
-    auto add = [&](int row0) -> bool {
-        uint32_t any = 0, bits = 0;
+    /* The next boxes of a window of 32 entries, a tile's number of them at most: lane u gets the first row of box u, -1 behind the last. */
+    unsigned todo = 0;
+    int sub = 0;                        /* box of a long block */
+    auto take = [&](int entry) -> int {
+        int row = -1;
+        if (p.per_entry == 1) {
+            for (int n = 0; todo && n < p.units; n++) {
+                const int v = __shfl_sync(0xffffffffu, entry, __ffs(todo) - 1) * p.k_block;     /* < seq_k */
+                todo &= todo - 1;
+                if (lane == n) row = v;
+            }
+        } else if (todo) {
+            const int v = __shfl_sync(0xffffffffu, entry, __ffs(todo) - 1) * p.k_block + sub * kTile;
+            if (lane == 0) row = v;
+            if (++sub == p.per_entry || v >= p.seq_k - kTile) {
+                sub = 0;
+                todo &= todo - 1;
+            }
+        }
+        return row;
+    };
+    /* What the mask says of their keys: keys 32 w + lane of the boxes side by side. Only looked at one step later. */
+    auto fetch = [&](int row, int flag[4]) {
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            const int key = 32 * w + lane;
-            bool valid = key < p.unit && row0 + key < p.seq_k;
-            if (valid && p.key_mask) valid = p.key_mask[row0 + key] != 0;
-            const uint32_t b = __ballot_sync(0xffffffffu, valid);
-            any |= b;
-            /* Word of the tile that these keys belong to (two boxes of 16 keys share one). */
-            if (lane == (filled * p.unit >> 5) + w) bits = p.unit == 16 ? b << (16 * (filled & 1)) : b;
+            const int key = 32 * w + lane, r0 = __shfl_sync(0xffffffffu, row, key >> p.unit_log), k = r0 + (key & (p.unit - 1));
+            flag[w] = 0;
+            if (r0 >= 0 && k < p.seq_k) flag[w] = p.key_mask ? p.key_mask[k] : 1;
         }
-        if (any == 0) return true;
-        if (32 * lane < kTile) key_bits |= bits;
-        if (lane == filled) row_of_unit = row0;
-        return ++filled < p.units || emit();
+    };
+    /* The boxes join the key tile at hand, except those of which the mask leaves nothing. */
+    auto add = [&](int row, int flag[4]) -> bool {
+        if (!p.key_mask && filled == 0 && __all_sync(0xffffffffu, lane >= p.units || (row >= 0 && row <= p.seq_k - p.unit))) {
+            key_bits = 0xFFFFFFFFu;
+            row_of_unit = row;
+            filled = p.units;
+            return emit(false);
+        }
+        uint32_t word = 0;              /* lane w < 4: keys [32 w, 32 w + 32) */
+        if (!p.key_mask) fetch(row, flag);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const uint32_t b = __ballot_sync(0xffffffffu, flag[w] != 0);
+            if (lane == w) word = b;
+        }
+        const bool some = p.unit == 16 ? (word & 0xFFFFu) && (word >> 16) : word != 0;
+        if (filled == 0 && __all_sync(0xffffffffu, lane >= 4 || some)) {
+            key_bits = word;
+            row_of_unit = row;
+            filled = p.units;
+            return emit(false);
+        }
+        const int words = p.unit >> 5;                          /* of a box; 0: half a word */
+        for (int u = 0; u < p.units; u++) {
+            const int r0 = __shfl_sync(0xffffffffu, row, u);
+            if (r0 < 0) break;
+            if (words == 0) {
+                const uint32_t half = (__shfl_sync(0xffffffffu, word, u >> 1) >> (16 * (u & 1))) & 0xFFFFu;
+                if (half == 0) continue;
+                if (lane == filled >> 1) key_bits |= half << (16 * (filled & 1));
+            } else {
+                const int at = lane - filled * words;           /* word of the box that this lane keeps */
+                const uint32_t v = __shfl_sync(0xffffffffu, word, (u * words + at) & 31);
+                const bool mine = at >= 0 && at < words;
+                if (!__any_sync(0xffffffffu, mine && v != 0)) continue;
+                if (mine) key_bits = v;
+            }
+            if (lane == filled) row_of_unit = r0;
+            if (++filled == p.units && !emit(false)) return false;
+        }
+        return true;
     };
 
-    for (int e = t.e0; ok && e < t.e1; e += 32) {
-        if (e > t.e0) entry = e + lane < t.e1 ? t.list[e + lane] : -1;
-        unsigned todo = __ballot_sync(0xffffffffu, entry >= 0 && entry < p.k_blocks);
-        while (ok && todo) {
-            const int src = __ffs(todo) - 1;
-            todo &= todo - 1;
-            const int row0 = __shfl_sync(0xffffffffu, entry, src) * p.k_block;     /* < seq_k */
-            for (int s = 0; ok && s < p.per_entry && row0 + s * kTile < p.seq_k; s++) ok = add(row0 + s * kTile);
+    const int step = item_step(p);
+    int item = first_item(p);
+    Tile t = tile_of(p, item, rank);
+    int entry = t.e0 + lane < t.e1 ? t.list[t.e0 + lane] : -1;
+    load_q(t);
+    while (ok) {
+        kcol = (t.head / p.group) * kHeadDim;
+        /* The first entries of the next query tile are on their way meanwhile. */
+        const int next_item = item < p.items - step ? item + step : -1;
+        Tile t2 = t;
+        int entry2 = -1;
+        if (next_item >= 0) {
+            t2 = tile_of(p, next_item, rank);
+            if (t2.e0 + lane < t2.e1) entry2 = t2.list[t2.e0 + lane];
         }
+        for (int e = t.e0; ok && e < t.e1; e += 32) {
+            if (e > t.e0) entry = e + lane < t.e1 ? t.list[e + lane] : -1;
+            todo = __ballot_sync(0xffffffffu, entry >= 0 && entry < p.k_blocks);
+            int row = take(entry), flag[4], next_flag[4];
+            if (p.key_mask) fetch(row, flag);
+            while (ok && __any_sync(0xffffffffu, row >= 0)) {
+                const int next_row = take(entry);
+                if (p.key_mask) fetch(next_row, next_flag);
+                ok = add(row, flag);
+                row = next_row;
+#pragma unroll
+                for (int w = 0; w < 4; w++) flag[w] = next_flag[w];
+            }
+        }
+        if (ok && filled > 0) ok = emit(false);
+        if (ok) ok = emit(true);
+        if (!ok || next_item < 0) break;
+        /* The last product with Q is done; a Q that none was made with has arrived. */
+        if (unused) ok = __all_sync(0xffffffffu, wait_bar(c, BAR_Q_FULL, (uint32_t)(loads_q - 1) & 1u, 402));
+        else if (j > 0) ok = __all_sync(0xffffffffu, wait_bar(c, BAR_K_EMPTY, (uint32_t)(j - 1) & 1u, 404));
+        if (!ok) break;
+        item = next_item;
+        t = t2;
+        entry = entry2;
+        load_q(t);
     }
-    if (ok && filled > 0) ok = emit();
-    /* (Without any block nobody else waits for Q, whose place the epilogue uses.) */
-    if (ok && j == 0 && t.e0 < t.e1) ok = __all_sync(0xffffffffu, wait_bar(c, BAR_Q_FULL, 0, 402));
-    if (ok) ok = emit();
     if (*c.abort_flag) {
         /* Nobody may be consuming any more: wait (bounded by the limit again) for the copies still in flight. */
         const unsigned long long t0 = global_ns();
         auto drain = [&](int bar, int n) {
             while (n > 0 && !mbar_try_wait(c.bars + bar * 8, (uint32_t)(n - 1) & 1u) && global_ns() - t0 < c.wait_ns + kDrainNs) {}
         };
-        drain(BAR_Q_FULL, t.e0 < t.e1);
-        drain(BAR_K_FULL, loads_k);
+        drain(BAR_Q_FULL, loads_q);
+        drain(BAR_K_FULL, j);
         drain(BAR_V_FULL, loads_v);
     }
 }
 
-/* Rows of V whose key does not count, cleared: four keys per lane. */
+/* Rows of V whose key does not count, cleared: 32 rows side by side where none
+ * of them does, else two at a time, half a warp each. */
 __device__ __forceinline__ void clear_rows(unsigned char *v, const volatile Meta *m, int lane) {
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    unsigned char *mine = v + ((lane >> 3) & 1) * kHalfBytes + (lane & 7) * 16;
 #pragma unroll 1
     for (int w = 0; w < 4; w++) {
-        if ((m->bits[w] >> lane) & 1u) continue;
-        const int row = 32 * w + lane;
-#pragma unroll 1
-        for (int half = 0; half < 2; half++)
-            for (int ch = 0; ch < 8; ch++)
-                *reinterpret_cast<uint4 *>(v + half * kHalfBytes + row * 128 + ch * 16) = make_uint4(0u, 0u, 0u, 0u);
+        uint32_t out = ~m->bits[w];
+        if (out == 0xFFFFFFFFu) {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                *reinterpret_cast<uint4 *>(v + (i >> 3) * kHalfBytes + w * 4096 + (i & 7) * 512 + lane * 16) = zero;
+            continue;
+        }
+        while (out) {
+            const int r0 = __ffs(out) - 1;
+            out &= out - 1;
+            const int r1 = out ? __ffs(out) - 1 : r0;
+            out &= out - 1;
+            *reinterpret_cast<uint4 *>(mine + (32 * w + (lane < 16 ? r0 : r1)) * 128) = zero;
+        }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -267,7 +390,7 @@ __device__ __forceinline__ void clear_rows(unsigned char *v, const volatile Meta
 
 __device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) { return ((uint64_t)hi << 32) | lo; }
 
-__device__ __forceinline__ void mma_issuer(const Ctx &c, uint32_t smem, unsigned char *smem_gen, uint32_t tmem,
+__device__ __forceinline__ void mma_issuer(const Ctx &c, const Params &p, uint32_t smem, unsigned char *smem_gen, uint32_t tmem,
                                            const volatile Meta *meta, int lane) {
     const uint32_t hi = (uint32_t)(make_desc(0, 0, kSbo) >> 32);
     const uint32_t lo_q = (uint32_t)make_desc(smem + kSmemQ, 1, 0), lo_k = (uint32_t)make_desc(smem + kSmemK, 1, 0);
@@ -278,7 +401,10 @@ __device__ __forceinline__ void mma_issuer(const Ctx &c, uint32_t smem, unsigned
     auto wait_all = [&](int bar, uint32_t par, int site) -> bool {
         return __all_sync(0xffffffffu, wait_bar(c, bar, par, site));
     };
-    auto state_of = [&](int j) -> uint32_t { return meta[j & (kMetaSlots - 1)].state; };
+    auto release = [&](int record) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(c.bars + (BAR_META_FREE + (record & (kMetaSlots - 1))) * 8);
+    };
     auto issue_qk = [&]() {
 #pragma unroll
         for (int ks = 0; ks < kHeadDim / 16; ks++) {
@@ -291,39 +417,43 @@ __device__ __forceinline__ void mma_issuer(const Ctx &c, uint32_t smem, unsigned
         }
     };
 
-    ok = wait_all(BAR_META, 0, 410);
-    bool more = ok && state_of(0) != 0u;
-    if (more) {
-        ok = wait_all(BAR_Q_FULL, 0, 411) && wait_all(BAR_K_FULL, 0, 412);
-        tc_fence_after();
-        if (ok) issue_qk();
-    }
-    for (int j = 0; ok && more; j++) {
-        const uint32_t par = (uint32_t)j & 1u;
-        if (!(ok = wait_all(BAR_V_FULL, par, 413))) break;
-        if (state_of(j) == 2u) clear_rows(smem_gen + kSmemV, meta + (j & (kMetaSlots - 1)), lane);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            if (!(ok = wait_all(BAR_P_FULL + h, par, 414 + h))) break;
+    int r = 0, j = 0, nq = 0;           /* records, key tiles whose scores were issued, query tiles with any */
+    for (int item = first_item(p); ok; item += item_step(p)) {
+        bool some = false;
+        while (ok) {
+            const int slot = r & (kMetaSlots - 1);
+            if (!(ok = wait_all(BAR_META + slot, (uint32_t)(r / kMetaSlots) & 1u, 410))) break;
+            const uint32_t state = meta[slot].state;
+            if (is_end(state)) {
+                if (some && leader) tc_commit(c.bars + BAR_O_DONE * 8);
+                nq += state == kEndUnused;
+                release(r++);
+                break;
+            }
+            const uint32_t par = (uint32_t)j & 1u;
+            if (!some && !(ok = wait_all(BAR_Q_FULL, (uint32_t)nq++ & 1u, 411))) break;
+            if (!(ok = wait_all(BAR_K_FULL, par, 412))) break;
             tc_fence_after();
+            issue_qk();
+            if (!(ok = wait_all(BAR_V_FULL, par, 413))) break;
+            if (state == kPartly) clear_rows(smem_gen + kSmemV, meta + slot, lane);
+            release(r++);
 #pragma unroll
-            for (int ks = 0; ks < 4; ks++)
-                if (leader)
-                    mma_ts(tmem + 128, tmem + h * 32 + ks * 8, desc64(lo_v + ((h * 64 + ks * 16) * 128 >> 4), hi), kIdescPV,
-                           j > 0 || h > 0 || ks > 0);
+            for (int h = 0; h < 2; h++) {
+                if (!(ok = wait_all(BAR_P_FULL + h, par, 414 + h))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++)
+                    if (leader)
+                        mma_ts(tmem + 128, tmem + h * 32 + ks * 8, desc64(lo_v + ((h * 64 + ks * 16) * 128 >> 4), hi), kIdescPV,
+                               some || h > 0 || ks > 0);
+            }
+            if (!ok) break;
+            if (leader) tc_commit(c.bars + BAR_V_EMPTY * 8);
+            some = true;
+            j++;
         }
-        if (!ok) break;
-        if (leader) tc_commit(c.bars + BAR_V_EMPTY * 8);
-        const int nx = j + 1;
-        if (!(ok = wait_all(BAR_META + (nx & (kMetaSlots - 1)), (uint32_t)(nx / kMetaSlots) & 1u, 416))) break;
-        more = state_of(nx) != 0u;
-        if (!more) {
-            if (leader) tc_commit(c.bars + BAR_O_DONE * 8);
-            break;
-        }
-        if (!(ok = wait_all(BAR_K_FULL, (uint32_t)nx & 1u, 417))) break;
-        tc_fence_after();
-        issue_qk();
+        if (item >= p.items - item_step(p)) break;
     }
     if (!ok) {
         /* Let what was issued finish before the tensor memory goes away. */
@@ -334,29 +464,45 @@ __device__ __forceinline__ void mma_issuer(const Ctx &c, uint32_t smem, unsigned
     }
 }
 
-/* The row's running state after all its keys. */
+/* The row's running state after all its keys, of one query tile. */
 struct RowState {
     float m, l;             /* reference (scaled log2 units) and sum */
     bool any;               /* O holds something */
     bool ok;
 };
 
-__device__ __forceinline__ RowState softmax_rows(const Ctx &c, const Params &p, const Tile &t, uint32_t tmem, const volatile Meta *meta) {
-    const int row = threadIdx.x & 127;
+/* Where a softmax warp stands: records read, key tiles, query tiles with any. */
+struct Progress {
+    int r, j, done;
+};
+
+__device__ __forceinline__ RowState softmax_rows(const Ctx &c, const Params &p, const Tile &t, uint32_t tmem, const volatile Meta *meta,
+                                                 Progress &at) {
+    const int row = threadIdx.x & 127, lane = threadIdx.x & 31;
     const uint32_t tS = tmem + ((uint32_t)(row & ~31) << 16), tO = tS + 128;
     const bool live = (row & ~31) < t.rows;              /* this warp has rows */
     const float sl2 = p.scale_log2;
     RowState st = {-INFINITY, 0.0f, false, true};
-    for (int j = 0;; j++) {
-        const int slot = j & (kMetaSlots - 1);
-        if (!(st.ok = __all_sync(0xffffffffu, wait_bar(c, BAR_META + slot, (uint32_t)(j / kMetaSlots) & 1u, 420)))) return st;
+    for (;; at.j++) {
+        const int slot = at.r & (kMetaSlots - 1);
+        if (!(st.ok = __all_sync(0xffffffffu, wait_bar(c, BAR_META + slot, (uint32_t)(at.r / kMetaSlots) & 1u, 420)))) return st;
+        at.r++;
         const uint32_t state = meta[slot].state;
-        if (state == 0u) break;
+        auto release = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(c.bars + (BAR_META_FREE + slot) * 8);
+        };
+        if (is_end(state)) {
+            release();
+            break;
+        }
+        const bool begin = !st.any;
         st.any = true;
-        if (!(st.ok = __all_sync(0xffffffffu, wait_bar(c, BAR_S_FULL, (uint32_t)j & 1u, 421)))) return st;
+        if (!(st.ok = __all_sync(0xffffffffu, wait_bar(c, BAR_S_FULL, (uint32_t)at.j & 1u, 421)))) return st;
         tc_fence_after();
         if (!live) {
             /* Rows that do not exist: whatever lies in P only meets rows of O that nobody reads. */
+            release();
             tc_fence_before();
             mbar_arrive(c.bars + BAR_P_FULL * 8);
             mbar_arrive(c.bars + (BAR_P_FULL + 1) * 8);
@@ -366,13 +512,14 @@ __device__ __forceinline__ RowState softmax_rows(const Ctx &c, const Params &p, 
 #pragma unroll
         for (int ch = 0; ch < 4; ch++) tmem_ld32(tS + ch * 32, s + ch * 32);
         tc_wait_ld();
-        if (state == 2u) {
+        if (state == kPartly) {
 #pragma unroll
             for (int ch = 0; ch < 4; ch++) {
                 const uint32_t bits = meta[slot].bits[ch];
                 if (bits != 0xFFFFFFFFu) mask_chunk(s + ch * 32, bits);
             }
         }
+        release();
         float mx8[8];
 #pragma unroll
         for (int a = 0; a < 8; a++) mx8[a] = fmaxf(__uint_as_float(s[2 * a]), __uint_as_float(s[2 * a + 1]));
@@ -384,12 +531,12 @@ __device__ __forceinline__ RowState softmax_rows(const Ctx &c, const Params &p, 
         }
         const float mx = fmaxf(max3(mx8[0], mx8[1], mx8[2]), max3(mx8[3], mx8[4], fmaxf(mx8[5], fmaxf(mx8[6], mx8[7]))));
         const float m_cand = fmaxf(st.m, mx * sl2);
-        if (j == 0) {
+        if (begin) {
             st.m = m_cand;
         } else {
             const bool need = m_cand > st.m + kRescaleThreshold;
             if (__any_sync(0xffffffffu, need)) {
-                /* PV(j - 1) is complete (it was issued before the QK that filled S) and PV(j) waits for this warp. */
+                /* The last product is complete (it was issued before the one that filled S), the next waits for this warp. */
                 const float alpha = need ? ex2(st.m - m_cand) : 1.0f;
                 if (need) {
                     st.l *= alpha;
@@ -418,50 +565,51 @@ __device__ __forceinline__ RowState softmax_rows(const Ctx &c, const Params &p, 
         st.l += (sum4[0] + sum4[2]) + (sum4[1] + sum4[3]);
     }
     if (st.any) {
-        st.ok = __all_sync(0xffffffffu, wait_bar(c, BAR_O_DONE, 0, 422));
+        st.ok = __all_sync(0xffffffffu, wait_bar(c, BAR_O_DONE, (uint32_t)at.done++ & 1u, 422));
         tc_fence_after();
     }
     return st;
 }
 
-/* O times f -> bf16 rows, through 8 KB of staging per warp (two halves of 32
- * rows x 128 bytes, 16-byte chunks swizzled by the row): a thread owns a row,
- * memory wants eight threads per 128 bytes of it. */
+/* O times f -> bf16 rows, through 4 KB of staging per warp (32 rows x 128
+ * bytes, 16-byte chunks swizzled by the row): a thread owns a row, memory wants
+ * eight threads per 128 bytes of it. */
 __device__ __forceinline__ void store_rows(const Params &p, const Tile &t, uint32_t tmem, float f, bool any, unsigned char *stage) {
     const int row = threadIdx.x & 127, lane = threadIdx.x & 31, row0 = row & ~31;
     if (row0 >= t.rows) return;
     const uint32_t tO = tmem + ((uint32_t)row0 << 16) + 128;
-    unsigned char *sw = stage + (row0 >> 5) * 8192;
+    unsigned char *sw = stage + (row0 >> 5) * 4096;
     uint16_t *out = p.out + (size_t)(t.q0 + row0) * p.ldo + (size_t)t.head * kHeadDim;
-    uint32_t o[128];
-    if (any) {
-#pragma unroll
-        for (int q = 0; q < 4; q++) tmem_ld32(tO + q * 32, o + q * 32);
-        tc_wait_ld();
-    }
-#pragma unroll
+#pragma unroll 1
     for (int half = 0; half < 2; half++) {
+        uint32_t o[64];
+        if (any) {
+            tmem_ld32(tO + half * 64, o);
+            tmem_ld32(tO + half * 64 + 32, o + 32);
+            tc_wait_ld();
+        } else {
+#pragma unroll
+            for (int i = 0; i < 64; i++) o[i] = 0u;
+        }
 #pragma unroll
         for (int ch = 0; ch < 8; ch++) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float a = __uint_as_float(o[64 * half + 8 * ch + 2 * e]), b = __uint_as_float(o[64 * half + 8 * ch + 2 * e + 1]);
-                w[e] = any && f != 0.0f ? cvt_bf16x2(a * f, b * f) : 0u;
+                const float a = __uint_as_float(o[8 * ch + 2 * e]), b = __uint_as_float(o[8 * ch + 2 * e + 1]);
+                w[e] = f != 0.0f ? cvt_bf16x2(a * f, b * f) : 0u;
             }
-            *reinterpret_cast<uint4 *>(sw + half * 4096 + lane * 128 + ((ch ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4 *>(sw + lane * 128 + ((ch ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-    }
-    __syncwarp();
-    const int ch = lane & 7;
-#pragma unroll
-    for (int half = 0; half < 2; half++) {
+        __syncwarp();
+        const int ch = lane & 7;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             const int r = k * 4 + (lane >> 3);
-            const uint4 v = *reinterpret_cast<const uint4 *>(sw + half * 4096 + r * 128 + ((ch ^ (r & 7)) << 4));
+            const uint4 v = *reinterpret_cast<const uint4 *>(sw + r * 128 + ((ch ^ (r & 7)) << 4));
             if (row0 + r < t.rows) *reinterpret_cast<uint4 *>(out + (size_t)r * p.ldo + half * 64 + ch * 8) = v;
         }
+        __syncwarp();
     }
 }
 
@@ -495,7 +643,6 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
     c.wait_ns = p.wait_ns;
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + kSmemBar + kOffTmemPtr);
     volatile Meta *meta = reinterpret_cast<volatile Meta *>(smem_gen + kSmemBar + kOffMeta);
-    const Tile t = tile_of(p, rank);
     /* The producer sets up the barriers and starts at once; it only tells the
      * other warps, which wait here for the barriers and the tensor memory. The
      * launch is stream-serialised by program: nothing may be read or written
@@ -503,9 +650,10 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
      * (What is read may be written until then: no load through the
      * non-coherent path, which takes memory as constant for the whole kernel.) */
     uint32_t tmem = 0;
-    if (warp == 4) {
+    const int shift = p.parts == 1 && blockIdx.x >= gridDim.x / 2 ? 2 : 0, producer_warp = 4 + shift, mma_warp = 5 + shift;
+    if (warp == producer_warp) {
         if (lane == 0) {
-            for (int b = 0; b < BAR_COUNT; b++) mbar_init(c.bars + b * 8, b == BAR_P_FULL || b == BAR_P_FULL + 1 ? 128 : 1);
+            for (int b = 0; b < BAR_COUNT; b++) mbar_init(c.bars + b * 8, b == BAR_P_FULL || b == BAR_P_FULL + 1 ? 128 : b >= BAR_META_FREE ? 5 : 1);
             *c.abort_flag = 0u;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -513,7 +661,7 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
         __syncwarp();
         asm volatile("barrier.cta.arrive.aligned 1, %0;" ::"n"(kThreads) : "memory");
     } else {
-        if (warp == 5) {
+        if (warp == mma_warp) {
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                          ::"r"(smem + kSmemBar + kOffTmemPtr), "r"(256u) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -528,12 +676,19 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
     RowState st = {-INFINITY, 0.0f, false, true};
     if (warp < 4) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        st = softmax_rows(c, p, t, tmem, meta);
-        if (p.parts == 1 && st.ok) store_rows(p, t, tmem, st.l != 0.0f ? 1.0f / st.l : 0.0f, st.any, smem_gen + kSmemQ);
+        Progress at = {0, 0, 0};
+        const int step = item_step(p);
+        for (int item = first_item(p);; item += step) {
+            const Tile t = tile_of(p, item, rank);
+            st = softmax_rows(c, p, t, tmem, meta, at);
+            if (!st.ok || p.parts > 1) break;
+            store_rows(p, t, tmem, st.l != 0.0f ? 1.0f / st.l : 0.0f, st.any, smem_gen + kSmemStage);
+            if (item >= p.items - step) break;
+        }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-        if (warp == 4) producer(c, p, t, &tmq, &tmk, &tmv, smem, meta, lane);
-        if (warp == 5) mma_issuer(c, smem, smem_gen, tmem, meta, lane);
+        if (warp == producer_warp) producer(c, p, rank, &tmq, &tmk, &tmv, smem, meta, lane);
+        if (warp == mma_warp) mma_issuer(c, p, smem, smem_gen, tmem, meta, lane);
         __syncwarp();
     }
 
@@ -543,14 +698,15 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
          * in shared memory; CTA r adds the columns [r, r + 1) * 128 / parts of
          * all of them. A row that no CTA has a key for stays zero. */
         const int row = threadIdx.x & 127;
-        float2 *ml = reinterpret_cast<float2 *>(smem_gen + kSmemBar + kOffMl);
+        const Tile t = tile_of(p, first_item(p), rank);
+        float2 *ml = reinterpret_cast<float2 *>(smem_gen + kSmemStage);
         if (warp < 4) ml[row] = make_float2(st.m, st.l);
         cluster_sync_all();
         if (warp < 4 && (row & ~31) < t.rows) {
             float m = -INFINITY, l = 0.0f;
-            for (int r = 0; r < p.parts; r++) m = fmaxf(m, ld_cluster_f2(map_to_cta(smem + kSmemBar + kOffMl + row * 8, r)).x);
+            for (int r = 0; r < p.parts; r++) m = fmaxf(m, ld_cluster_f2(map_to_cta(smem + kSmemStage + row * 8, r)).x);
             for (int r = 0; r < p.parts; r++) {
-                const float2 o = ld_cluster_f2(map_to_cta(smem + kSmemBar + kOffMl + row * 8, r));
+                const float2 o = ld_cluster_f2(map_to_cta(smem + kSmemStage + row * 8, r));
                 if (o.y != 0.0f) l += o.y * ex2(o.x - m);
             }
             const float f = st.ok && st.any && st.l != 0.0f ? ex2(st.m - m) / l : 0.0f;
@@ -596,7 +752,7 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 5) {
+    if (warp == mma_warp) {
         tc_fence_after();
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
@@ -651,6 +807,7 @@ int launch_attention_blocks_sm100(const BlockAttnArgs &a) {
     p.k_blocks = a.k_blocks;
     p.tiles = (p.q_block + kTile - 1) / kTile;
     p.unit = a.k_block < kTile ? a.k_block : kTile;
+    p.unit_log = p.unit == 16 ? 4 : p.unit == 32 ? 5 : p.unit == 64 ? 6 : 7;
     p.units = kTile / p.unit;
     p.per_entry = a.k_block < kTile ? 1 : a.k_block / kTile;
     p.scale_log2 = a.scale * 1.4426950408889634f;
@@ -658,6 +815,8 @@ int launch_attention_blocks_sm100(const BlockAttnArgs &a) {
     p.wait_ns = wait_limit_ns();
     const long long items = (long long)a.heads * a.q_blocks * p.tiles;
     const long long key_tiles = ((long long)a.list_len * p.per_entry + p.units - 1) / p.units;
+    p.per_head = a.q_blocks * p.tiles;
+    p.items = (int)items;
     p.parts = choose_parts(items, key_tiles, g.sm_count);
     /* Whole key tiles per part, where every entry names a block. */
     const int tile_entries = p.units > 1 ? p.units : 1;
@@ -668,7 +827,8 @@ int launch_attention_blocks_sm100(const BlockAttnArgs &a) {
         !make_tensor_map(&tmv, a.v, a.seq_k, a.kv_heads * kHeadDim, a.ldv, p.unit))
         return IRIS_B200_ECUDA;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.q_blocks * p.tiles * p.parts), (unsigned)a.heads);
+    const long long slots = 2LL * g.sm_count;
+    cfg.gridDim = dim3((unsigned)(p.parts > 1 ? items * p.parts : items < slots ? items : slots));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kSmemBytes;
     cfg.stream = g.stream;

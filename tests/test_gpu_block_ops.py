@@ -464,6 +464,34 @@ def test_attention_tensor_kernel_more_tiles_than_fit_at_once(lib, sq, heads, n, 
     check_attention(lib, sq, 2900, heads, 2, 128, n, qb, 64, TCGEN05, masked, 0, junk)
 
 
+@pytest.mark.parametrize("kb,n", [(16, 11), (32, 6), (64, 3), (128, 2), (256, 2)])
+def test_attention_tensor_kernel_tiles_without_keys_among_others(lib, kb, n):
+    """Empty lists and lists of masked blocks only, in runs, between tiles with keys, several tiles to a CTA."""
+    sq, sk, heads = 3900, 2100, 20
+    nq, nk = -(-sq // 128), -(-sk // kb)
+    gen = torch.Generator().manual_seed(kb)
+    q, k, v = (randn(kb + i, r, D if i else heads * D).bfloat16() for i, r in enumerate((sq, sk, sk)))
+    mask = (torch.rand(sk, generator=gen) < 0.97).int()
+    mask[512:1024] = 0                       # whole blocks of every size
+    k[mask == 0], v[mask == 0] = NAN, NAN
+    lists = random_lists(kb + 7, heads, nq, nk, n)
+    what = torch.randint(0, 4, (heads, nq), generator=gen)
+    masked = torch.arange(512 // kb, 1024 // kb)
+    for h in range(heads):
+        for i in range(nq):
+            if what[h, i] == 0:
+                lists[h, i] = -1
+            elif what[h, i] == 1:
+                lists[h, i] = masked[torch.randint(0, len(masked), (n,), generator=gen)].int()
+    got = run_attention(lib, q, k, v, heads, 1, D, mask, lists, 128, kb, TCGEN05)
+    want, mag = ref.attention(q, k, v, heads, 1, D, D ** -0.5, mask, lists, 128, kb)
+    assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * mag).all()
+    for h in range(heads):
+        for i in range(nq):
+            if what[h, i] < 2:
+                assert (got[i * 128:(i + 1) * 128, h * D:(h + 1) * D] == 0).all()
+
+
 @pytest.mark.parametrize("sq,heads,n", [(1, 8, 40), (300, 3, 6), (100, 2, 40)])
 def test_attention_tensor_kernel_growing_scores(lib, sq, heads, n):
     """Scores that rise from block to block, so that the running maximum moves and O is rescaled."""
