@@ -10,6 +10,10 @@ Tolerances, all derived from the arithmetic:
   attention   one bf16 rounding of every probability (2^-8 of sum p |v|) and of the result (2^-8 of it); 2^-12 of
               sum p |v| covers fp32 scores (a 128-long dot product times scale, |s| < 16: 2^-13) and exponentials (2^-21)
 """
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -318,6 +322,18 @@ def test_block_select_many_equal_scores(lib, nq, nk, kv):
         assert torch.equal(run_select(lib, qm, km, counts, topk, first, last), want)
 
 
+def test_block_select_unaligned_means(lib):
+    """Means at an odd word: the same lists."""
+    nq, nk, heads, kv = 5, 300, 4, 2
+    qm, km = randn(1, nq, heads, D), randn(2, nk, kv, D)
+    a, b = torch.zeros(qm.numel() + 1).cuda(), torch.zeros(km.numel() + 1).cuda()
+    a[1:], b[1:] = qm.flatten(), km.flatten()
+    out = torch.zeros(heads, nq, 20, dtype=torch.int32).cuda()
+    assert lib.iris_b200_block_select(ptr(out), ptr(a, 1), ptr(b, 1), None, nq, nk, heads, kv, D, 20, 1, 1) == 0
+    done(lib)
+    assert torch.equal(out.cpu(), ref.select(qm, km, None, 20, 1, 1))
+
+
 def test_block_select_values_that_are_not_finite(lib):
     qm, km = randn(1, 2, 1, 128), randn(2, 20, 1, 128)
     km[4] = NAN                              # ranks last, but before nothing
@@ -610,6 +626,69 @@ def test_the_operators_together(lib):
     a, b = out.double(), dense.cpu().double()
     mag = ref.attention(q.cpu(), k.cpu(), v.cpu(), heads, kv, D, D ** -0.5, mask, lists, qb, kb)[1]
     assert ((a - b).abs() <= 2.0 ** -7 * b.abs() + (2.0 ** -7 + 2.0 ** -11) * mag).all()
+
+
+@pytest.mark.parametrize("kernel", [GENERIC, TCGEN05, AUTO])
+@pytest.mark.parametrize("sq", [1, 100])
+def test_attention_blocks_larger_than_the_sequences(lib, kernel, sq):
+    """One block holds all keys, one all queries: the dense attention."""
+    check_attention(lib, sq, 300, 2, 1, 128, 1, 2 ** 31 - 1, 2 ** 30, kernel)
+    check_attention(lib, sq, 300, 2, 1, 128, 3, 2 ** 30, 2 ** 31 - 128, kernel, masked=True)
+
+
+FIRST_CALLS = """
+import sys, torch
+sys.path[:0] = [%r, %r]
+import __graft_entry__ as ge
+lib = ge.load_package().load()
+lib.init()
+s = torch.cuda.Stream()
+D, seq, heads = 128, 1000, 2
+x = torch.randn(seq, 3 * heads * D, device="cuda").bfloat16()
+q, k, out = (torch.zeros(seq, heads * D, device="cuda").bfloat16() for _ in range(3))
+pos = torch.randint(0, 90, (seq, 3), dtype=torch.int32, device="cuda")
+cos, sin = torch.zeros(seq, 64, device="cuda"), torch.zeros(seq, 64, device="cuda")
+qm, km = torch.zeros(8, heads, D, device="cuda"), torch.zeros(16, heads, D, device="cuda")
+lists = torch.zeros(heads, 8, 5, dtype=torch.int32, device="cuda")
+plan = lib.rope_axes((32, 48, 48), None, 256.0, False, D)
+p = lambda t: t.data_ptr()
+torch.cuda.synchronize()
+
+def run():
+    ld, w = 3 * heads * D, heads * D
+    assert lib.iris_b200_use_stream(torch.cuda.current_stream().cuda_stream) == 0
+    rc = lib.iris_b200_rope_axes_tables(p(cos), p(sin), p(pos), plan, seq, D)
+    rc |= lib.iris_b200_qk_norm_rope_axes(p(q), w, p(k), w, p(x), p(x) + 2 * w, ld, None, None, p(pos), plan, seq, heads, heads, D, 0.0, 0)
+    rc |= lib.iris_b200_block_means(p(qm), None, p(q), w, seq, heads, D, 128, None)
+    rc |= lib.iris_b200_block_means(p(km), None, p(k), w, seq, heads, D, 64, None)
+    rc |= lib.iris_b200_block_select(p(lists), p(qm), p(km), None, 8, 16, heads, heads, D, 5, 0, 0)
+    rc |= lib.iris_b200_attention_blocks(p(out), w, p(q), w, p(k), w, p(x) + 4 * w, ld, seq, seq, heads, heads, D, 0.1, None, p(lists), 5,
+                                         128, 64, 0)
+    rc |= lib.iris_b200_attention_blocks(p(out), w, p(q), w, p(k), w, p(x) + 4 * w, ld, 1, seq, heads, heads, D, 0.1, None, p(lists), 5,
+                                         1, 64, 0)
+    assert rc == 0, lib.iris_b200_last_error()
+
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    run()
+g.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (cos, sin, q, k, qm, km, lists, out)]
+with torch.cuda.stream(s):
+    run()
+torch.cuda.synchronize()
+assert got[7].abs().sum() > 0
+assert all(torch.equal(a, b) for a, b in zip(got, (cos, sin, q, k, qm, km, lists, out)))
+lib.check()
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing that a first call sets up is closed to a capture."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS % (os.path.dirname(here), here)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
 
 
 def test_offsets_that_pass_32_bits(lib):
