@@ -770,6 +770,64 @@ def test_calls_behind_one_another_see_what_the_last_one_wrote(lib):
         assert all(torch.equal(x, y) for x, y in zip(b, alone[n % 3])), n
 
 
+def test_large_calls_on_several_streams_at_once(lib):
+    """Two attentions over key blocks that each fill the device, single rows, lists and the dense attention side by side: what
+    they give alone."""
+    heads, seq, qb, kb, n = 16, 4000, 128, 64, 9
+    nq, nk = -(-seq // qb), -(-seq // kb)
+    home, side = torch.cuda.current_stream(), [torch.cuda.Stream() for _ in range(4)]
+
+    def inputs(seed):
+        q, k, v = (randn(seed + i, seq, heads * D).bfloat16().cuda() for i in range(3))
+        qm, km = torch.zeros(nq, heads, D).cuda(), torch.zeros(nk, heads, D).cuda()
+        return q, k, v, qm, km, torch.zeros(heads, nq, n, dtype=torch.int32).cuda(), torch.zeros_like(q)
+
+    def blocks(x):
+        q, k, v, qm, km, lists, out = x
+        w = heads * D
+        rc = lib.iris_b200_block_means(ptr(qm), None, ptr(q), w, seq, heads, D, qb, None)
+        rc |= lib.iris_b200_block_means(ptr(km), None, ptr(k), w, seq, heads, D, kb, None)
+        rc |= lib.iris_b200_block_select(ptr(lists), ptr(qm), ptr(km), None, nq, nk, heads, heads, D, n, 1, 0)
+        rc |= lib.iris_b200_attention_blocks(ptr(out), w, ptr(q), w, ptr(k), w, ptr(v), w, seq, seq, heads, heads, D, D ** -0.5, None,
+                                             ptr(lists), n, qb, kb, TCGEN05)
+        return rc
+
+    def rows(x):
+        q, k, v, qm, km, lists, out = x
+        w = heads * D
+        rc = lib.iris_b200_block_means(ptr(km), None, ptr(k), w, seq, heads, D, kb, None)
+        rc |= lib.iris_b200_block_select(ptr(lists), ptr(qm), ptr(km), None, 1, nk, heads, heads, D, n, 0, 0)
+        rc |= lib.iris_b200_attention_blocks(ptr(out), w, ptr(q), w, ptr(k), w, ptr(v), w, 1, seq, heads, heads, D, D ** -0.5, None,
+                                             ptr(lists), n, 1, kb, AUTO)
+        return rc
+
+    def dense(x):
+        q, k, v, _, _, _, out = x
+        w = heads * D
+        return lib.iris_b200_attention_ex(ptr(out), w, ptr(q), ptr(k), ptr(v), w, seq, seq, heads, heads, D, D ** -0.5, 0, None, 0)
+
+    work = list(zip((blocks, blocks, rows, dense), (inputs(10 * i) for i in range(4)), side))
+    torch.cuda.synchronize()
+    alone = []
+    for fn, x, _ in work:
+        assert fn(x) == 0
+        done(lib)
+        alone.append((x[5].clone(), x[6].clone()))
+        x[6].zero_()
+    torch.cuda.synchronize()
+    try:
+        for _ in range(12):
+            for fn, x, s in work:
+                assert lib.iris_b200_use_stream(s.cuda_stream) == 0
+                assert fn(x) == 0
+        torch.cuda.synchronize()
+    finally:
+        lib.iris_b200_use_stream(home.cuda_stream)
+    done(lib)
+    for (_, x, _), (lists, out) in zip(work, alone):
+        assert torch.equal(x[5], lists) and torch.equal(x[6], out)
+
+
 def test_captured_and_replayed(lib):
     """A captured run of the chain gives on replay, with new inputs, what eager calls give; two graphs replayed on two streams
     at once do not disturb one another."""
