@@ -509,6 +509,8 @@ k_block_select(const __grid_constant__ Select p) {
     const int rank = p.ctas > 1 ? (int)sm100::cluster_cta_rank() : 0;
     const int g = blockIdx.y;
     const long long r0 = (long long)(blockIdx.x / (unsigned)p.ctas) * p.rows;
+    /* Before a CTA's shared memory is written by others it has to have started: told here, asked before the first store. */
+    if (p.ctas > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int b0 = rank * p.slice, b1 = b0 + p.slice < p.k_blocks ? b0 + p.slice : p.k_blocks;
     auto block_at = [&](int j0) -> const float * {
@@ -539,8 +541,8 @@ k_block_select(const __grid_constant__ Select p) {
 #pragma unroll
         for (int k = 0; k < 4; k++) dst[k * 32] = (double)v[k];
     }
-    if (p.ctas > 1) sm100::cluster_sync_all();           /* every CTA has started: its shared memory may be written */
-    else __syncthreads();
+    __syncthreads();
+    if (p.ctas > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     for (int j0 = b0 + warp * 8; j0 < b1; j0 += kSelWarps * 8) {
         const Block<HD> k = next;
         next.load(block_at(j0 + kSelWarps * 8), lane);       /* under the products of this tile */
