@@ -726,10 +726,22 @@ extern "C" int iris_b200_block_select(int *list, const float *q_means, const flo
     while (p.ctas < g_max_ctas && tiles_of() * kv_heads * p.ctas * 2 <= 2LL * g.sm_count && k_blocks >= p.ctas * 2 * kSelWarps * 8)
         p.ctas *= 2;
     if (p.ctas > 8 && smem_of() > kWideSmem) p.ctas = 8;
+    /* Fewer rows per cluster where CTAs are left: choosing for a row takes
+     * longer than its scores. A row is not shared by so many warps that they
+     * have less than two blocks a lane. (30 query blocks x 5 heads x 120
+     * blocks: 16 rows of a CTA 11.0 us, eight 7.3, four 8.3; 5 x 20 heads x
+     * 549 blocks, two rows 11.8 us, one 8.9; 8 x 8 heads x 222 blocks, eight
+     * rows 9.9 us, four 7.7, two 7.4, one 8.5.) */
+    auto team_of = [](int own) { return own >= kSelWarps ? 1 : own > 2 ? 2 : own > 1 ? 4 : 8; };
+    while (p.rows > 1 && tiles_of() * kv_heads * p.ctas * 2 <= 2LL * g.sm_count) {
+        const int half = (p.rows + 1) / 2, own = (half + p.ctas - 1) / p.ctas, team = team_of(own);
+        if (own >= (p.rows + p.ctas - 1) / p.ctas || (team > 1 && k_blocks < 64 * team)) break;
+        p.rows = half;
+    }
     while (p.rows > 1 && smem_of() > kSelSmem) p.rows--;
     const size_t smem = smem_of();
     p.slice = ((k_blocks + p.ctas - 1) / p.ctas + 7) / 8 * 8;
-    p.team = p.own_rows >= kSelWarps ? 1 : p.own_rows > 2 ? 2 : p.own_rows > 1 ? 4 : 8;
+    p.team = team_of(p.own_rows);
     const long long clusters = tiles_of();
     if (clusters * p.ctas > INT_MAX) return bad(op, "too many query blocks");
     cudaLaunchConfig_t cfg = {};
