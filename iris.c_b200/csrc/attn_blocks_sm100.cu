@@ -340,10 +340,12 @@ __device__ __forceinline__ void producer(const Ctx &c, const Params &p, int rank
         }
         if (ok && filled > 0) ok = emit(false);
         if (ok) ok = emit(true);
+        /* A Q that no product is made with has to arrive before the next one is asked for, and before the CTA
+         * leaves: nobody else waits for it, and its shared memory may be another CTA's by then. */
+        if (ok && unused) ok = __all_sync(0xffffffffu, wait_bar(c, BAR_Q_FULL, (uint32_t)(loads_q - 1) & 1u, 402));
         if (!ok || next_item < 0) break;
-        /* The last product with Q is done; a Q that none was made with has arrived. */
-        if (unused) ok = __all_sync(0xffffffffu, wait_bar(c, BAR_Q_FULL, (uint32_t)(loads_q - 1) & 1u, 402));
-        else if (j > 0) ok = __all_sync(0xffffffffu, wait_bar(c, BAR_K_EMPTY, (uint32_t)(j - 1) & 1u, 404));
+        /* The last product with Q is done. */
+        if (!unused && j > 0) ok = __all_sync(0xffffffffu, wait_bar(c, BAR_K_EMPTY, (uint32_t)(j - 1) & 1u, 404));
         if (!ok) break;
         item = next_item;
         t = t2;
