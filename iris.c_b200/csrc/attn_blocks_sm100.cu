@@ -53,7 +53,8 @@
  * last probability to its next scores 1 400.
  *
  * Every wait on a barrier is bounded as in the dense kernel; a CTA that gives
- * up still takes part in the cluster's barriers.
+ * up still takes part in the cluster's barriers, and before it leaves it waits
+ * (bounded again) for its copies and products in flight.
  */
 #include "attn_tc.cuh"
 #include "common.cuh"
@@ -175,8 +176,25 @@ __device__ __forceinline__ Tile tile_of(const Params &p, int item, int rank) {
 __device__ __forceinline__ int first_item(const Params &p) { return p.parts > 1 ? (int)(blockIdx.x / (unsigned)p.parts) : (int)blockIdx.x; }
 __device__ __forceinline__ int item_step(const Params &p) { return p.parts > 1 ? p.items : (int)gridDim.x; }
 
-__device__ __forceinline__ void producer(const Ctx &c, const Params &p, int rank, const CUtensorMap *mq, const CUtensorMap *mk,
-                                         const CUtensorMap *mv, uint32_t smem, volatile Meta *meta, int lane) {
+/* How many loads of Q, K and V a producer has issued. */
+struct Loads {
+    int q, k, v;
+};
+
+/* In a CTA that gave up nobody may have waited for the last loads: they arrive
+ * (bounded by the limit again) before its shared memory goes away. */
+__device__ __forceinline__ void drain_loads(const Ctx &c, const Loads &n) {
+    const unsigned long long t0 = global_ns();
+    auto drain = [&](int bar, int loads) {
+        while (loads > 0 && !mbar_try_wait(c.bars + bar * 8, (uint32_t)(loads - 1) & 1u) && global_ns() - t0 < c.wait_ns + kDrainNs) {}
+    };
+    drain(BAR_Q_FULL, n.q);
+    drain(BAR_K_FULL, n.k);
+    drain(BAR_V_FULL, n.v);
+}
+
+__device__ __forceinline__ Loads producer(const Ctx &c, const Params &p, int rank, const CUtensorMap *mq, const CUtensorMap *mk,
+                                          const CUtensorMap *mv, uint32_t smem, volatile Meta *meta, int lane) {
     int r = 0, j = 0;                   /* records published, key tiles loaded */
     int loads_q = 0, loads_v = 0;
     int filled = 0;                     /* boxes of the key tile being put together; lane u holds the first row of box u */
@@ -352,16 +370,7 @@ __device__ __forceinline__ void producer(const Ctx &c, const Params &p, int rank
         entry = entry2;
         load_q(t);
     }
-    if (*c.abort_flag) {
-        /* Nobody may be consuming any more: wait (bounded by the limit again) for the copies still in flight. */
-        const unsigned long long t0 = global_ns();
-        auto drain = [&](int bar, int n) {
-            while (n > 0 && !mbar_try_wait(c.bars + bar * 8, (uint32_t)(n - 1) & 1u) && global_ns() - t0 < c.wait_ns + kDrainNs) {}
-        };
-        drain(BAR_Q_FULL, loads_q);
-        drain(BAR_K_FULL, j);
-        drain(BAR_V_FULL, loads_v);
-    }
+    return {loads_q, j, loads_v};
 }
 
 /* Rows of V whose key does not count, cleared: 32 rows side by side where none
@@ -457,13 +466,15 @@ __device__ __forceinline__ void mma_issuer(const Ctx &c, const Params &p, uint32
         }
         if (item >= p.items - item_step(p)) break;
     }
-    if (!ok) {
-        /* Let what was issued finish before the tensor memory goes away. */
-        if (leader) tc_commit(c.bars + BAR_DRAIN * 8);
-        const uint32_t bar = c.bars + BAR_DRAIN * 8;
-        const unsigned long long t0 = global_ns();
-        while (!mbar_try_wait(bar, 0) && global_ns() - t0 < c.wait_ns + kDrainNs) {}
-    }
+}
+
+/* In a CTA that gave up: the products issued so far (by the lane that the same election chose) end before their operands and
+ * the tensor memory go away. */
+__device__ __forceinline__ void drain_products(const Ctx &c) {
+    if (elect_one()) tc_commit(c.bars + BAR_DRAIN * 8);
+    __syncwarp();
+    const unsigned long long t0 = global_ns();
+    while (!mbar_try_wait(c.bars + BAR_DRAIN * 8, 0) && global_ns() - t0 < c.wait_ns + kDrainNs) {}
 }
 
 /* The row's running state after all its keys, of one query tile. */
@@ -676,6 +687,7 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     RowState st = {-INFINITY, 0.0f, false, true};
+    Loads loads = {0, 0, 0};
     if (warp < 4) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         Progress at = {0, 0, 0};
@@ -689,7 +701,7 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-        if (warp == producer_warp) producer(c, p, rank, &tmq, &tmk, &tmv, smem, meta, lane);
+        if (warp == producer_warp) loads = producer(c, p, rank, &tmq, &tmk, &tmv, smem, meta, lane);
         if (warp == mma_warp) mma_issuer(c, p, smem, smem_gen, tmem, meta, lane);
         __syncwarp();
     }
@@ -754,6 +766,12 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
     }
     tc_fence_before();
     __syncthreads();
+    /* Any warp may have given up, at any time: whether one has is known for the whole CTA only here. */
+    if (*c.abort_flag) {
+        if (warp == producer_warp) drain_loads(c, loads);
+        if (warp == mma_warp) drain_products(c);
+        __syncwarp();
+    }
     if (warp == mma_warp) {
         tc_fence_after();
         __syncwarp();

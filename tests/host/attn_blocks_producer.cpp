@@ -90,7 +90,8 @@ static volatile Meta g_meta[kMetaSlots];
 static int g_issued[3], g_waited[3];            /* copies of Q, K, V */
 static long long g_bytes[3], g_expected[3];
 static bool g_with_keys;
-static int g_records;
+static int g_records, g_give_up;                /* records published; how many of them the other warps live to see */
+static volatile uint32_t g_abort[2];
 static int g_unit;                              /* rows of a box of K or V */
 struct Box {
     int which, load, x, row;
@@ -108,8 +109,9 @@ static int which_of(uint32_t bar) {
 }
 
 namespace sm100 {
-/* Everything that is waited for has happened; what the producer itself waits for of its copies is noted. */
+/* Everything that is waited for has happened, as long as nobody gave up; what the producer itself waits for of its copies is noted. */
 static uint32_t mbar_try_wait(uint32_t bar, uint32_t parity) {
+    if (g_abort[0] && (int)(bar / 8) != BAR_Q_FULL && (int)(bar / 8) != BAR_K_FULL && (int)(bar / 8) != BAR_V_FULL) return 0;
     if (t_lane != 0) return 1;
     const int b = (int)(bar / 8);
     if (b == BAR_Q_FULL || b == BAR_K_FULL || b == BAR_V_FULL) {
@@ -136,11 +138,14 @@ static void mbar_arrive(uint32_t bar) {
         g_with_keys = false;
         return;
     }
-    /* The products of the tile wait for its K and V, the first of a query tile for Q. */
-    if (!g_with_keys) g_waited[0] = g_issued[0];
+    /* The products of the tile wait for its K and V, the first of a query tile for Q; who has given up waits for nothing. */
+    if (g_records > g_give_up) g_abort[0] = 1u;
+    if (!g_abort[0]) {
+        if (!g_with_keys) g_waited[0] = g_issued[0];
+        g_waited[1]++;
+        g_waited[2]++;
+    }
     g_with_keys = true;
-    g_waited[1]++;
-    g_waited[2]++;
     printf("keys %s %08x %08x %08x %08x\n", m.state == kWhole ? "whole" : "partly", m.bits[0], m.bits[1], m.bits[2], m.bits[3]);
 }
 static std::atomic_flag g_lock = ATOMIC_FLAG_INIT;
@@ -154,13 +159,14 @@ static void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint
 }  // namespace sm100
 }  // namespace iris_b200
 
-/* Arguments: seq_q seq_k heads group list_len q_block k_block rank parts part_len block grid, then the list, then seq_k mask words (or none). */
+/* Arguments: seq_q seq_k heads group list_len q_block k_block rank parts part_len block grid, the record at which the others
+ * give up (0: none), then the list, then seq_k mask words (or none). */
 int main(int argc, char **argv) {
     using namespace iris_b200;
     using namespace iris_b200::attn_blocks;
     std::vector<int> a;
     for (int i = 1; i < argc; i++) a.push_back(atoi(argv[i]));
-    if (a.size() < 12) return 2;
+    if (a.size() < 13) return 2;
     Params p = {};
     p.seq_q = a[0];
     p.seq_k = a[1];
@@ -186,19 +192,21 @@ int main(int argc, char **argv) {
     p.items = p.heads * p.per_head;
     p.wait_ns = 1;
     const size_t nlist = (size_t)p.heads * p.q_blocks * p.list_len;
-    if (a.size() != 12 + nlist && a.size() != 12 + nlist + (size_t)p.seq_k) return 2;
-    p.list = a.data() + 12;
-    p.key_mask = a.size() > 12 + nlist ? a.data() + 12 + nlist : nullptr;
+    if (a.size() != 13 + nlist && a.size() != 13 + nlist + (size_t)p.seq_k) return 2;
+    p.list = a.data() + 13;
+    p.key_mask = a.size() > 13 + nlist ? a.data() + 13 + nlist : nullptr;
     unsigned int status[8] = {};
-    uint32_t abort_word[2] = {};
+    g_give_up = a[12] ? a[12] - 1 : 1 << 30;
     p.status = status;
     const CUtensorMap maps[3] = {{0}, {1}, {2}};
     std::vector<std::thread> warp;
     for (int lane = 0; lane < kLanes; lane++)
         warp.emplace_back([&, lane] {
             t_lane = lane;
-            Ctx c = {0, abort_word, status, 1};
-            producer(c, p, rank, &maps[0], &maps[1], &maps[2], 0, g_meta, lane);
+            Ctx c = {0, g_abort, status, 1};
+            const Loads n = producer(c, p, rank, &maps[0], &maps[1], &maps[2], 0, g_meta, lane);
+            __syncwarp();
+            if (*c.abort_flag) drain_loads(c, n);
         });
     for (auto &t : warp) t.join();
     for (const Box &b : g_boxes)
@@ -207,5 +215,5 @@ int main(int argc, char **argv) {
         printf("copies %c issued %d waited %d\n", "QKV"[w], g_issued[w], g_waited[w]);
         if (g_bytes[w] != g_expected[w]) return 4;
     }
-    return abort_word[0] ? 3 : 0;
+    return g_abort[0] != (a[12] != 0) ? 3 : 0;
 }
