@@ -6,9 +6,11 @@
  * 512, any alignment, any block sizes). A CTA owns up to eight consecutive
  * queries of one head inside one query block, one warp per query; keys of the
  * listed blocks are staged in shared memory 32 at a time, each lane scores one
- * key, and the softmax runs with a running maximum and sum in fp32. Rows of
- * masked keys are staged as zeros, so whatever they hold never meets a zero
- * probability. It is the form the tensor-core kernel is checked against.
+ * key, and the softmax runs with a running maximum and sum in fp32; the
+ * probabilities meet V in fp32 too, as in the kernel for rows with a list of
+ * their own (only the tensor cores want them as bf16). Rows of masked keys are
+ * staged as zeros, so whatever they hold never meets a zero probability. It is
+ * the form the tensor-core kernel is checked against.
  *
  * The automatic choice: rows with a list of their own go to the kernel that
  * reads keys into registers (attn_blocks_row.cu: 1 row 14.7 us against 19.1 on
@@ -92,12 +94,10 @@ k_attention_blocks_any(const BlockAttnArgs a, int tiles_per_block) {
             for (int o = 16; o > 0; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
             l = l * alpha + ps;
             m = mnew;
-            /* The probabilities meet V as bf16, as in the tensor-core kernel; their sum keeps fp32. */
-            const float pb = bf_lo(cvt_bf16x2(p, 0.0f));
 #pragma unroll
             for (int t = 0; t < kMaxHeadDim / 32; t++) acc[t] *= alpha;
             for (int j = 0; j < kKeysPerTile; j++) {
-                const float pj = __shfl_sync(0xffffffffu, pb, j);
+                const float pj = __shfl_sync(0xffffffffu, p, j);
                 const uint16_t *vr = vs + j * hd;
 #pragma unroll
                 for (int t = 0; t < kMaxHeadDim / 32; t++) {
