@@ -4,9 +4,10 @@
  *
  * k_block_means reads every element once and is bound by HBM. A CTA owns one
  * block of rows and 256 columns, 32 lanes x 16 bytes; its eight warps take
- * every eighth row. A thread adds up to eight rows in fp32 and joins these
- * partial sums, and then the warps', in fp64, so that a mean is off by no more
- * than the rounding of a few eight-row sums. 16 889 rows x 32 heads in blocks
+ * every eighth row. A thread adds up to eight rows in fp32, an eighth of each
+ * (exact in fp32 for every bf16 value, and eight of the largest do not overflow),
+ * and joins these partial sums, and then the warps', in fp64, so that a mean is
+ * off by no more than the rounding of eight-row sums. 16 889 rows x 32 heads in blocks
  * of 128 (141 MB) take 23.8 us, 5.9 TB/s; 4608 x 30 in blocks of 64 (37 MB)
  * 8.9 us, less than two waves of CTAs.
  *
@@ -93,10 +94,12 @@ k_block_means(float *means, int *counts, const uint16_t *x, int ldx, int seq, in
         for (int i = 0; i < 8; i++) s[i] = 0.0f;
 #pragma unroll
         for (int i = 0; i < kMeanRun; i++) {
-            s[0] += bf_lo(v[i].x); s[1] += bf_hi(v[i].x);
-            s[2] += bf_lo(v[i].y); s[3] += bf_hi(v[i].y);
-            s[4] += bf_lo(v[i].z); s[5] += bf_hi(v[i].z);
-            s[6] += bf_lo(v[i].w); s[7] += bf_hi(v[i].w);
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s[2 * e] = fmaf(bf_lo(w[e]), 1.0f / kMeanRun, s[2 * e]);
+                s[2 * e + 1] = fmaf(bf_hi(w[e]), 1.0f / kMeanRun, s[2 * e + 1]);
+            }
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) acc[i] += (double)s[i];
@@ -113,7 +116,7 @@ k_block_means(float *means, int *counts, const uint16_t *x, int ldx, int seq, in
         sum += part[w][threadIdx.x];
         total += part_n[w];
     }
-    if (c < width) means[(size_t)blockIdx.x * width + c] = total ? (float)(sum / total) : 0.0f;
+    if (c < width) means[(size_t)blockIdx.x * width + c] = total ? (float)(sum * kMeanRun / total) : 0.0f;
     if (counts && blockIdx.y == 0 && threadIdx.x == 0) counts[blockIdx.x] = total;
 }
 
