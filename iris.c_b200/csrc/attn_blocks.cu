@@ -62,7 +62,8 @@ k_attention_blocks_any(const BlockAttnArgs a, int tiles_per_block) {
         if (b < 0 || b >= a.k_blocks) continue;
         const long long first = (long long)b * a.k_block;
         const int rows = (int)(a.seq_k - first < a.k_block ? a.seq_k - first : a.k_block);
-        for (int k0 = 0; k0 < rows; k0 += kKeysPerTile) {
+        /* (64 bits: k0 passes the last row by more than a 31-bit count has room for.) */
+        for (long long k0 = 0; k0 < rows; k0 += kKeysPerTile) {
             __syncthreads();
             if (warp == 0) {
                 const bool ok = k0 + lane < rows && (!a.key_mask || a.key_mask[first + k0 + lane] != 0);
