@@ -84,6 +84,7 @@ static constexpr int kRegsSoftmax = 184, kRegsOther = 72;    /* 128 * 184 + 128 
 static constexpr int kMaxParts = 8;
 static constexpr unsigned long long kDrainNs = 100000000ull;      /* for work in flight, beyond the wait limit */
 static constexpr int kMetaSlots = 4;
+static constexpr uint32_t kReadsPerBeat = 8192;
 static constexpr uint32_t kSbo = 1024 / 16;              /* 8 rows of 128 B, in 16-byte units */
 static constexpr uint32_t kVLbo = kHalfBytes / 16;       /* next 64 dims */
 static constexpr uint32_t kIdescQK = idesc_bf16(128, 128);
@@ -102,9 +103,10 @@ enum {
 };
 static constexpr int kOffTmemPtr = BAR_COUNT * 8;
 static constexpr int kOffAbort = kOffTmemPtr + 4;
+static constexpr int kOffBeat = kOffAbort + 4;           /* grows while the producer reads on */
 static constexpr int kOffMeta = 160;                     /* kMetaSlots x 32 bytes */
 static constexpr int kSmemBytes = kSmemBar + kOffMeta + kMetaSlots * 32;
-static_assert(kOffAbort + 4 <= kOffMeta, "barrier block");
+static_assert(kOffBeat + 4 <= kOffMeta, "barrier block");
 static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
 
 /* What the producer publishes: the key tiles of a query tile, and its end. */
@@ -136,16 +138,26 @@ struct Params {
 /* The bounded wait of the dense kernel, except that it first looks at the clock
  * after 64 tries: reading it takes about a thousand cycles, which a wait that is
  * nearly over should not pay (16 896 rows x 32 heads over 64 blocks: 1210 us
- * with the clock read on entry, 1060 us so). */
+ * with the clock read on entry, 1060 us so). READER: the wait is for a record,
+ * which may be millions of list entries away: it begins anew while the producer
+ * shows that it reads on. */
+template <bool READER = false>
 __device__ __forceinline__ bool wait_bar(const Ctx &c, int idx, uint32_t parity, int site) {
     const uint32_t bar = c.bars + idx * 8;
     unsigned long long t0 = 0;
+    uint32_t beat = 0;
     for (uint32_t spin = 1;; spin++) {
         if (mbar_try_wait(bar, parity)) return true;
         if (spin % 64u != 0) continue;
         if (*c.abort_flag) return false;
         if (t0 == 0) t0 = global_ns();
         if (global_ns() - t0 > c.wait_ns || spin > (1u << 26)) {
+            if (READER && c.abort_flag[1] != beat) {
+                beat = c.abort_flag[1];
+                t0 = 0;
+                spin = 0;
+                continue;
+            }
             give_up(c, site, parity);
             return false;
         }
@@ -254,6 +266,14 @@ __device__ __forceinline__ Loads producer(const Ctx &c, const Params &p, int ran
         return true;
     };
 
+    /* A sign of life (and a look at the others') every so many reads without a key tile, each the latency of a load: milliseconds. */
+    uint32_t reads = 0;
+    auto read_on = [&]() -> bool {
+        if (++reads % kReadsPerBeat != 0) return true;
+        if (lane == 0) c.abort_flag[1] = reads;
+        return __all_sync(0xffffffffu, *c.abort_flag == 0u);
+    };
+
     /* The next boxes of a window of 32 entries, a tile's number of them at most: lane u gets the first row of box u, -1 behind the last. */
     unsigned todo = 0;
     int sub = 0;                        /* box of a long block */
@@ -324,7 +344,7 @@ __device__ __forceinline__ Loads producer(const Ctx &c, const Params &p, int ran
             if (lane == filled) row_of_unit = r0;
             if (++filled == p.units && !emit(false)) return false;
         }
-        return true;
+        return read_on();
     };
 
     const int step = item_step(p);
@@ -344,6 +364,7 @@ __device__ __forceinline__ Loads producer(const Ctx &c, const Params &p, int ran
         }
         for (int e = t.e0; ok && e < t.e1; e += 32) {
             if (e > t.e0) entry = e + lane < t.e1 ? t.list[e + lane] : -1;
+            ok = read_on();
             todo = __ballot_sync(0xffffffffu, entry >= 0 && entry < p.k_blocks);
             int row = take(entry), flag[4], next_flag[4];
             if (p.key_mask) fetch(row, flag);
@@ -433,7 +454,7 @@ __device__ __forceinline__ void mma_issuer(const Ctx &c, const Params &p, uint32
         bool some = false;
         while (ok) {
             const int slot = r & (kMetaSlots - 1);
-            if (!(ok = wait_all(BAR_META + slot, (uint32_t)(r / kMetaSlots) & 1u, 410))) break;
+            if (!(ok = __all_sync(0xffffffffu, wait_bar<true>(c, BAR_META + slot, (uint32_t)(r / kMetaSlots) & 1u, 410)))) break;
             const uint32_t state = meta[slot].state;
             if (is_end(state)) {
                 if (some && leader) tc_commit(c.bars + BAR_O_DONE * 8);
@@ -498,7 +519,7 @@ __device__ __forceinline__ RowState softmax_rows(const Ctx &c, const Params &p, 
     RowState st = {-INFINITY, 0.0f, false, true};
     for (;; at.j++) {
         const int slot = at.r & (kMetaSlots - 1);
-        if (!(st.ok = __all_sync(0xffffffffu, wait_bar(c, BAR_META + slot, (uint32_t)(at.r / kMetaSlots) & 1u, 420)))) return st;
+        if (!(st.ok = __all_sync(0xffffffffu, wait_bar<true>(c, BAR_META + slot, (uint32_t)(at.r / kMetaSlots) & 1u, 420)))) return st;
         at.r++;
         const uint32_t state = meta[slot].state;
         auto release = [&]() {
@@ -667,7 +688,7 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
     if (warp == producer_warp) {
         if (lane == 0) {
             for (int b = 0; b < BAR_COUNT; b++) mbar_init(c.bars + b * 8, b == BAR_P_FULL || b == BAR_P_FULL + 1 ? 128 : b >= BAR_META_FREE ? 5 : 1);
-            *c.abort_flag = 0u;
+            c.abort_flag[0] = c.abort_flag[1] = 0u;      /* and the beat */
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }

@@ -26,11 +26,11 @@ class Call:
         self.gpu = [t.cuda() for t in (self.q, self.k, self.v, lists)]
         self.out = torch.zeros(sq + 1, heads * D, dtype=torch.bfloat16, device="cuda")
 
-    def launch(self, lib):
+    def launch(self, lib, mask=None):
         q, k, v, lists = self.gpu
         self.out.fill_(7.0)
         assert lib.iris_b200_attention_blocks(ptr(self.out), self.heads * D, ptr(q), self.heads * D, ptr(k), D, ptr(v), D, self.sq,
-                                              self.sk, self.heads, 1, D, D ** -0.5, None, ptr(lists), lists.shape[2], self.qb,
+                                              self.sk, self.heads, 1, D, D ** -0.5, ptr(mask), ptr(lists), lists.shape[2], self.qb,
                                               self.kb, TCGEN05) == 0
 
     def check(self):
@@ -89,3 +89,29 @@ def test_limits_of_the_length_of_a_copy(lib):
     call.launch(lib)
     done(lib)
     call.check()
+
+
+@pytest.mark.parametrize("skip,masked", [(1 << 25, False), (1 << 21, True)])
+def test_reading_a_list_may_take_longer_than_the_limit(lib, skip, masked):
+    """Tens of milliseconds of entries that name nothing, or a block that is masked as a whole, under a limit of ten: the
+    other warps see that the producer reads on."""
+    call = Call(100, 1, skip)
+    mask = None
+    if masked:
+        call.gpu[3][..., :skip] = 3
+        mask = torch.ones(call.sk, dtype=torch.int32)
+        mask[3 * call.kb:4 * call.kb] = 0
+        mask = mask.cuda()
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    try:
+        lib.iris_b200_set_wait_limit_us(10000)
+        for _ in range(2):
+            a.record()
+            call.launch(lib, mask)
+            b.record()
+            assert status(lib) == 0
+            assert a.elapsed_time(b) > 20.0
+            call.check()
+    finally:
+        lib.iris_b200_set_wait_limit_us(0)
+    done(lib)
