@@ -1,5 +1,6 @@
 """ctypes declarations of every entry point in include/*.h."""
 import ctypes as C
+import operator
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -192,10 +193,14 @@ class Lib:
         return p
 
     def rope_axes(self, dims, scales, theta, one_progression, head_dim):
-        """The rotation plan of iris_b200_rope_axes_plan."""
+        """The rotation plan of iris_b200_rope_axes_plan; scales: one for every axis, or None (or empty) for all 1."""
         plan = RopeAxes()
         n = len(dims)
-        rc = self.iris_b200_rope_axes_plan(plan, (INT * n)(*dims), (C.c_double * n)(*scales) if scales else None, n, theta,
+        scales = [] if scales is None else [float(s) for s in scales]
+        if scales and len(scales) != n:
+            raise ValueError("%d scales for %d axes" % (len(scales), n))
+        scale = (C.c_double * n)(*scales) if scales else None
+        rc = self.iris_b200_rope_axes_plan(plan, (INT * n)(*[operator.index(d) for d in dims]), scale, n, theta,
                                            int(one_progression), head_dim)
         if rc:
             raise IrisB200Error("iris_b200 error %d: %s" % (rc, self.iris_b200_strerror(rc).decode()))
