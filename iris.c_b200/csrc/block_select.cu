@@ -306,8 +306,13 @@ __device__ __forceinline__ uint32_t high_of(const unsigned long long *key) { ret
  * by one warp, more by a search over their bits. The chosen keys of the bin are
  * turned into all ones, and everything above the bin is taken.
  * WORDS > 0: a lane holds that many upper words in registers, which covers the
- * run, and every pass over them is straight-line code (with the words read from
- * shared memory in loops, a row of 264 blocks took 5 us instead of 3.3). */
+ * run, and every pass over them is straight-line code. It is compiled for the
+ * multiples of four up to sixteen, as places that hold no word cost as much as
+ * those that do: 132 query blocks x 32 heads over 128 / 256 / 384 / 512 blocks
+ * take 14.9 / 23.5 / 32.2 / 40.8 us, with sixteen words alone 18.0 / 25.5 / 33.1 /
+ * 40.5, with the words read from shared memory in loops (WORDS 0) 16.1 / 26.3 /
+ * 36.3 / 46.2. (Even counts: half a microsecond less where they round up by less,
+ * for twice the code.) Longer runs go through the loops: 544 blocks 49.8 us. */
 template <int WORDS>
 __device__ __forceinline__ void choose(const Select &p, Team t, unsigned long long *keys, TeamScratch &sc, int *list) {
     const int lane = threadIdx.x & 31;
@@ -584,8 +589,10 @@ k_block_select(const __grid_constant__ Select p) {
             const int words = ((p.k_blocks + p.team - 1) / p.team + 31) / 32;        /* of a lane */
             if (words <= 4)
                 choose<4>(p, t, mine, sc, list);
-            else if (words <= 9)
-                choose<9>(p, t, mine, sc, list);
+            else if (words <= 8)
+                choose<8>(p, t, mine, sc, list);
+            else if (words <= 12)
+                choose<12>(p, t, mine, sc, list);
             else if (words <= 16)
                 choose<16>(p, t, mine, sc, list);
             else
