@@ -4,8 +4,11 @@
  *
  * Pair j of a head turns by p[s, axis(j)] * f_j. f_j / 2 pi is kept as a
  * 64-bit fraction of a turn F_j, so the phase of a row is p * F_j modulo 2^64:
- * whole turns fall off by themselves, for any sign and size of p, with an
- * error of |p| 2^-65 turns; there is no range reduction and no table. Of the
+ * whole turns fall off by themselves, for any sign and size of p; there is no
+ * range reduction and no table. The fraction is cut, not rounded, and comes from
+ * a frequency in long double, so the phase is off by up to |p| 2^-64 (1 + r f_j /
+ * 2 pi) turns with r = 5 roundings and the logarithm of the power of theta, 19 at
+ * most for theta 1e6: at |p| 2^31 and f_j 1 that is 4.7e-10 turns (2.9e-9 rad). Of the
  * phase the top 32 bits are used (2^-32 turns = 1.5e-9 rad): the two highest
  * give the quadrant after rounding, the rest an angle a within pi / 4 on which
  * a + a^3 S(a^2) and 1 - a^2 / 2 + a^4 C(a^2), with quadratics S and C of least
