@@ -391,6 +391,12 @@ __device__ __forceinline__ Loads producer(const Ctx &c, const Params &p, int ran
         entry = entry2;
         load_q(t);
     }
+    /* The softmax warps see the end of the last products by a barrier of its own; their arrivals at these two come before
+     * the CTA leaves as well. */
+    if (ok && j > 0) {
+        const uint32_t par = (uint32_t)(j - 1) & 1u;
+        __all_sync(0xffffffffu, wait_bar(c, BAR_K_EMPTY, par, 405) && wait_bar(c, BAR_V_EMPTY, par, 406));
+    }
     return {loads_q, j, loads_v};
 }
 

@@ -88,6 +88,7 @@ using namespace attn_blocks;
 
 static volatile Meta g_meta[kMetaSlots];
 static int g_issued[3], g_waited[3];            /* copies of Q, K, V */
+static int g_emptied[3];                        /* key tiles whose products with K, V somebody saw to their end */
 static long long g_bytes[3], g_expected[3];
 static bool g_with_keys;
 static int g_records, g_give_up;                /* records published; how many of them the other warps live to see */
@@ -114,6 +115,11 @@ static uint32_t mbar_try_wait(uint32_t bar, uint32_t parity) {
     if (g_abort[0] && (int)(bar / 8) != BAR_Q_FULL && (int)(bar / 8) != BAR_K_FULL && (int)(bar / 8) != BAR_V_FULL) return 0;
     if (t_lane != 0) return 1;
     const int b = (int)(bar / 8);
+    /* (Arrivals of the tensor cores: one for every key tile whose products were issued.) */
+    if (b == BAR_K_EMPTY || b == BAR_V_EMPTY) {
+        const int w = b == BAR_K_EMPTY ? 1 : 2;
+        if (((g_issued[w] - 1) & 1) == (int)parity) g_emptied[w] = g_issued[w];
+    }
     if (b == BAR_Q_FULL || b == BAR_K_FULL || b == BAR_V_FULL) {
         const int w = which_of(bar);
         if (((g_issued[w] - 1) & 1) == (int)parity) g_waited[w] = std::max(g_waited[w], g_issued[w]);
@@ -213,6 +219,7 @@ int main(int argc, char **argv) {
         printf("box %c %d %d %d %u\n", "QKV"[b.which], b.load, b.x, b.row, b.at);
     for (int w = 0; w < 3; w++) {
         printf("copies %c issued %d waited %d\n", "QKV"[w], g_issued[w], g_waited[w]);
+        if (w) printf("products %c issued %d waited %d\n", "QKV"[w], g_issued[w], g_emptied[w]);
         if (g_bytes[w] != g_expected[w]) return 4;
     }
     return g_abort[0] != (a[12] != 0) ? 3 : 0;

@@ -22,7 +22,8 @@ def producer(tmp_path_factory):
                     os.path.join(HERE, "host", "attn_blocks_producer.cpp")], check=True)
 
     def run(seq_q, seq_k, heads, q_block, k_block, lists, mask=None, group=1, rank=0, parts=1, part_len=None, block=0, grid=1, give_up=0):
-        """lists [heads][q_blocks][n]; the loads of Q, K and V as {tensor: (issued, waited)}, and the query tiles of the CTA: for
+        """lists [heads][q_blocks][n]; the loads of Q, K and V, and the products
+        with K and V, as {name: (issued, waited)}, and the query tiles of the CTA: for
         each its key tiles as 128 key rows, None where the key does not count."""
         n = len(lists[0][0])
         args = [seq_q, seq_k, heads, group, n, q_block, k_block, rank, parts, n if part_len is None else part_len, block, grid, give_up]
@@ -33,8 +34,8 @@ def producer(tmp_path_factory):
         loads, records, boxes = {}, [], {"Q": [], "K": [], "V": []}
         for line in done.stdout.splitlines():
             w = line.split()
-            if w[0] == "copies":
-                loads[w[1]] = (int(w[3]), int(w[5]))
+            if w[0] in ("copies", "products"):
+                loads[w[1] if w[0] == "copies" else w[1] + " products"] = (int(w[3]), int(w[5]))
             elif w[0] == "box":
                 boxes[w[1]].append(tuple(int(x) for x in w[2:]))
             else:
@@ -127,4 +128,4 @@ def test_key_tiles_hold_the_keys_of_the_lists(producer, k_block, n, masked, step
 def test_no_copy_outlives_a_cta_that_gives_up(producer, give_up):
     """The other warps stop at any record, the last ones among them: the copies that nobody waits for any more are drained."""
     loads, _ = producer(128 * 3, 1000, 1, 128, 64, [[[0, 1, 2, 3, 4], [5, 6, -1, -1, -1], [7, 8, 9, 10, 11]]], give_up=give_up)
-    assert loads["K"][0] >= 1 and all_waited(loads), loads
+    assert loads["K"][0] >= 1 and all(loads[t][0] == loads[t][1] for t in "QKV"), loads
