@@ -138,10 +138,13 @@ struct Params {
 /* The bounded wait of the dense kernel, except that it first looks at the clock
  * after 64 tries: reading it takes about a thousand cycles, which a wait that is
  * nearly over should not pay (16 896 rows x 32 heads over 64 blocks: 1210 us
- * with the clock read on entry, 1060 us so). READER: the wait is for a record,
- * which may be millions of list entries away: it begins anew while the producer
- * shows that it reads on. */
-template <bool READER = false>
+ * with the clock read on entry, 1060 us so).
+ * A record may be millions of list entries away. The MMA warp's wait for one
+ * (kReader) begins anew while the producer shows that it reads on, and the
+ * softmax warps (kFollower), which wait for the same record, leave the clock to
+ * the MMA warp: they see its flag. */
+enum WaitKind { kPlain, kReader, kFollower };
+template <WaitKind KIND = kPlain>
 __device__ __forceinline__ bool wait_bar(const Ctx &c, int idx, uint32_t parity, int site) {
     const uint32_t bar = c.bars + idx * 8;
     unsigned long long t0 = 0;
@@ -150,17 +153,19 @@ __device__ __forceinline__ bool wait_bar(const Ctx &c, int idx, uint32_t parity,
         if (mbar_try_wait(bar, parity)) return true;
         if (spin % 64u != 0) continue;
         if (*c.abort_flag) return false;
-        if (t0 == 0) t0 = global_ns();
-        if (global_ns() - t0 > c.wait_ns || spin > (1u << 26)) {
-            if (READER && c.abort_flag[1] != beat) {
+        if (spin <= (1u << 26)) {
+            if (KIND == kFollower) continue;
+            if (t0 == 0) t0 = global_ns();
+            if (global_ns() - t0 <= c.wait_ns) continue;
+            if (KIND == kReader && c.abort_flag[1] != beat) {
                 beat = c.abort_flag[1];
                 t0 = 0;
                 spin = 0;
                 continue;
             }
-            give_up(c, site, parity);
-            return false;
         }
+        give_up(c, site, parity);
+        return false;
     }
 }
 
@@ -193,9 +198,17 @@ struct Loads {
     int q, k, v;
 };
 
-/* In a CTA that gave up nobody may have waited for the last loads: they arrive
- * (bounded by the limit again) before its shared memory goes away. */
-__device__ __forceinline__ void drain_loads(const Ctx &c, const Loads &n) {
+/* What has to have happened before the shared memory goes away, looked at
+ * behind the CTA's last barrier. The tensor cores have arrived for the last
+ * products with K and V (the softmax warps saw their end by a barrier of a later
+ * commit, which does not order the arrivals); in a CTA that gave up, where nobody
+ * may have waited for the last loads, those are in (bounded by the limit again). */
+__device__ __forceinline__ void settle_loads(const Ctx &c, const Loads &n) {
+    if (!*c.abort_flag) {
+        const uint32_t par = (uint32_t)(n.k - 1) & 1u;
+        if (n.k > 0 && wait_bar(c, BAR_K_EMPTY, par, 405)) wait_bar(c, BAR_V_EMPTY, par, 406);
+        return;
+    }
     const unsigned long long t0 = global_ns();
     auto drain = [&](int bar, int loads) {
         while (loads > 0 && !mbar_try_wait(c.bars + bar * 8, (uint32_t)(loads - 1) & 1u) && global_ns() - t0 < c.wait_ns + kDrainNs) {}
@@ -391,12 +404,6 @@ __device__ __forceinline__ Loads producer(const Ctx &c, const Params &p, int ran
         entry = entry2;
         load_q(t);
     }
-    /* The softmax warps see the end of the last products by a barrier of its own; their arrivals at these two come before
-     * the CTA leaves as well. */
-    if (ok && j > 0) {
-        const uint32_t par = (uint32_t)(j - 1) & 1u;
-        __all_sync(0xffffffffu, wait_bar(c, BAR_K_EMPTY, par, 405) && wait_bar(c, BAR_V_EMPTY, par, 406));
-    }
     return {loads_q, j, loads_v};
 }
 
@@ -460,7 +467,7 @@ __device__ __forceinline__ void mma_issuer(const Ctx &c, const Params &p, uint32
         bool some = false;
         while (ok) {
             const int slot = r & (kMetaSlots - 1);
-            if (!(ok = __all_sync(0xffffffffu, wait_bar<true>(c, BAR_META + slot, (uint32_t)(r / kMetaSlots) & 1u, 410)))) break;
+            if (!(ok = __all_sync(0xffffffffu, wait_bar<kReader>(c, BAR_META + slot, (uint32_t)(r / kMetaSlots) & 1u, 410)))) break;
             const uint32_t state = meta[slot].state;
             if (is_end(state)) {
                 if (some && leader) tc_commit(c.bars + BAR_O_DONE * 8);
@@ -525,7 +532,7 @@ __device__ __forceinline__ RowState softmax_rows(const Ctx &c, const Params &p, 
     RowState st = {-INFINITY, 0.0f, false, true};
     for (;; at.j++) {
         const int slot = at.r & (kMetaSlots - 1);
-        if (!(st.ok = __all_sync(0xffffffffu, wait_bar<true>(c, BAR_META + slot, (uint32_t)(at.r / kMetaSlots) & 1u, 420)))) return st;
+        if (!(st.ok = __all_sync(0xffffffffu, wait_bar<kFollower>(c, BAR_META + slot, (uint32_t)(at.r / kMetaSlots) & 1u, 420)))) return st;
         at.r++;
         const uint32_t state = meta[slot].state;
         auto release = [&]() {
@@ -794,12 +801,9 @@ k_attention_blocks_sm100(const __grid_constant__ CUtensorMap tmq, const __grid_c
     tc_fence_before();
     __syncthreads();
     /* Any warp may have given up, at any time: whether one has is known for the whole CTA only here. */
-    if (*c.abort_flag) {
-        if (warp == producer_warp) drain_loads(c, loads);
-        if (warp == mma_warp) drain_products(c);
-        __syncwarp();
-    }
+    if (warp == producer_warp) settle_loads(c, loads);
     if (warp == mma_warp) {
+        if (*c.abort_flag) drain_products(c);
         tc_fence_after();
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");

@@ -10,7 +10,7 @@
  * Prints the records (key tiles with their valid keys, ends of query tiles), the
  * copies (tensor, number of the load, coordinates, place in shared memory), and
  * how many loads of Q, K and V were issued and how many of them somebody waited
- * for before the producer returned.
+ * for before the CTA may leave.
  */
 #include <algorithm>
 #include <atomic>
@@ -212,7 +212,7 @@ int main(int argc, char **argv) {
             Ctx c = {0, g_abort, status, 1};
             const Loads n = producer(c, p, rank, &maps[0], &maps[1], &maps[2], 0, g_meta, lane);
             __syncwarp();
-            if (*c.abort_flag) drain_loads(c, n);
+            settle_loads(c, n);
         });
     for (auto &t : warp) t.join();
     for (const Box &b : g_boxes)
