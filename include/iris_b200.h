@@ -451,10 +451,14 @@ int iris_b200_block_select(int *list, const float *q_means, const float *k_means
  * list_len <= 2^30, heads <= 65535. kernel: one of IRIS_B200_KERNEL_*; the
  * tcgen05 kernel serves head_dim 128, k_block 16, 32, 64 or a multiple of 128,
  * strides in multiples of 8 and 16-byte aligned pointers, the general one
- * everything up to head_dim 512. The automatic choice has a third kernel for
- * q_block 1 or a single query row (tokens at the end of a long cache), with
- * head_dim 64, 128 or 256, any k_block, the same strides and alignment of q, k
- * and v. */
+ * everything up to head_dim 512, on the CUDA cores: a prompt takes it some 200
+ * times as long (4608 rows x 30 heads, head_dim 64: 22 ms), so a caller who would
+ * rather know names IRIS_B200_KERNEL_TCGEN05, which then answers
+ * IRIS_B200_EUNSUPPORTED. The automatic choice has a third kernel for q_block 1
+ * or a single query row (tokens at the end of a long cache), with head_dim 64,
+ * 128 or 256, any k_block, the same strides and alignment of q, k and v.
+ * Softmax and sums are fp32 and the result is rounded once; the tcgen05 kernel
+ * also rounds each probability to bf16, the type of V. */
 int iris_b200_attention_blocks(uint16_t *out, int ldo, const uint16_t *q, int ldq,
                                const uint16_t *k, int ldk, const uint16_t *v, int ldv,
                                int seq_q, int seq_k, int heads, int kv_heads, int head_dim, float scale,

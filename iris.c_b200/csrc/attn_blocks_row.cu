@@ -17,8 +17,9 @@
  * then in the first one.
  *
  * Bound by HBM where the lists of a call do not fit in L2: one row of 32 heads
- * over 64 blocks of 64 keys each, 67 MB, takes 14.7 us back to back (4.6 TB/s);
- * with head_dim 256, 134 MB, 24.4 us, so that 67 MB more cost 9.6 us (7.0
+ * over 64 blocks of 64 keys each reads 67 MB (61 MB of different rows, where four
+ * heads share a key head and their lists overlap) in 14.8 us back to back (4.5
+ * TB/s); with head_dim 256, 134 MB, 24.4 us, so that 67 MB more cost 9.6 us (7.0
  * TB/s) and 5 us are launch, list, first loads and joining. The tensor-core
  * kernel takes 19.1 us for the former, and for 256 rows of 32 heads over 32
  * blocks, out of L2, 893 us against 712. Half as many loads per warp and twice

@@ -37,8 +37,12 @@
  * front of S. MMA order: QK(0) PV(0) QK(1) PV(1) ...; each PV in two halves of
  * 64 keys as the softmax hands them over. The softmax is that of the dense
  * kernel: base 2, the reference value of a row moves only when its maximum
- * grows by more than 8, P rounded to bf16 for the MMA while the row sum keeps
- * fp32. A row without any key yields zeros.
+ * grows by more than 8. P is rounded to bf16, since the operands of one
+ * kind::f16 product have one type and V is bf16; the row sum keeps fp32. That
+ * rounding is 0.0016 of a result (root mean square of a bf16 rounding over a
+ * mantissa) beside the 0.0017 of the result's own: together 0.0023 against 64
+ * bits, and more bits would take a second product. A row without any key yields
+ * zeros.
  *
  * Records: the producer hands the tiles of keys and the end of every query
  * tile to the softmax and MMA warps through a ring of four records, which all
@@ -46,8 +50,10 @@
  * parities count key tiles (Q, O: query tiles with keys) of the whole CTA.
  *
  * Bound by the chain scores -> softmax -> product: 16 896 rows x 32 heads over
- * 64 blocks of 64 keys take 1 010 to 1 040 us (1.09 to 1.12 PFLOP/s), where the
- * products alone would take 690. Per pair of key tiles an SM spends about 3 700
+ * 64 blocks of 64 keys take 1 020 to 1 030 us in a short run (1.10 to 1.11
+ * PFLOP/s) and 1 180 in a run of seconds, at 1 600 MHz under the 1000 W cap, where
+ * the products alone would take 690 and 810 at the burst and the sustained rate;
+ * tensor pipe and exponential unit are busy for 55 % of the cycles. Per pair of key tiles an SM spends about 3 700
  * cycles, 2 048 of them in products and, beside them, 2 048 in exponentials;
  * the two CTAs alternate, a softmax takes 1 700 cycles and the way from its
  * last probability to its next scores 1 400.

@@ -23,7 +23,7 @@
  * the CTA that chooses for the row. One to eight warps then find the topk-th
  * largest key of a row, by a histogram and within its bin by rank, and write
  * the chosen blocks in ascending order, equal keys from the lowest index.
- * 132 query blocks x 32 heads over 264 blocks take 25.4 us: products about 14
+ * 132 query blocks x 32 heads over 264 blocks take 26.2 us: products about 14
  * (8 at the rate of the fp64 matrix pipe), the choice 3.3 a row, two rows a
  * warp. One query block of 32 heads on 8 key heads over 2048 blocks 11.9 us:
  * latency of the cluster's barriers, the loads and the choice. tf32 products
